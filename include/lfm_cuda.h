@@ -341,6 +341,115 @@ lfm_status lfm_attention_prefill(const float* q_dev, uint32_t q_stride, const vo
                                  uint32_t ctx, uint32_t start, uint32_t n, float* out_dev, uint32_t out_stride,
                                  void* stream);
 
+/* ---- attention over session caches (no reference counterpart) ---------
+ * Operators for sessions whose cache outgrows or shares its context: windowed
+ * attention, attention over a shared prefix, attention weights accumulated per
+ * cache position, and eviction by those weights. They take any head layout:
+ * q and out rows hold `heads` x head_dim values, a cache slot is
+ * [kv_heads][ctx][head_dim] (the engine's layout) and query head h reads KV
+ * head h / (heads / kv_heads).
+ *
+ * A query at position p sees position j when j <= p and (window == 0 or
+ * p - j < window or j < sinks). Only positions that some query of the call
+ * sees are read; a cache row that no query of the call sees may hold anything,
+ * NaN included. A value that is not finite in a row that is seen spreads to
+ * the queries that see it and may spread to the other queries of the call.
+ *
+ * All calls are asynchronous on `stream`, allocate nothing and may be captured
+ * into a graph. Pointers are device pointers of the current device, 16-byte
+ * aligned; strides are in elements and a multiple of 16 bytes. What a kernel
+ * finds wrong in device-side arguments it skips and reports through
+ * lfm_attention_status. */
+#define LFM_ATTN_F32 0u  /* fp32 q and out over fp16 caches (the engine's) */
+#define LFM_ATTN_F16 1u  /* fp16 q, out and caches */
+#define LFM_ATTN_BF16 2u /* bf16 q, out and caches */
+#define LFM_ATTN_MAX_GROUP 8u
+
+typedef struct lfm_attn_shape {
+  uint32_t dtype;    /* LFM_ATTN_* */
+  uint32_t heads;    /* kv_heads x 1..8 */
+  uint32_t kv_heads; /* 1..1024 */
+  uint32_t head_dim; /* 64 or 128 */
+  uint32_t ctx;      /* positions of a cache slot, 1..2^24 */
+  float scale;       /* of q.k, finite and > 0; 0 means 1/sqrt(head_dim) */
+} lfm_attn_shape;
+
+/* Prompt attention with a sliding window and sinks: queries at positions
+ * start .. start + n - 1 of one slot, start + n <= ctx, n <= 2^20. q row t at
+ * q + t * q_stride (the first heads x head_dim values of a longer row, such as
+ * the engine's fused q|k|v rows), out likewise. lse [n][heads] fp32 (may be
+ * null) receives the natural log of the sum of exponentials of each row's
+ * scaled scores, which lfm_attention_weights takes. */
+lfm_status lfm_attention_window(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* k_cache,
+                                const void* v_cache, uint32_t start, uint32_t n, uint32_t window, uint32_t sinks,
+                                void* out, uint64_t out_stride, float* lse, void* stream);
+
+/* One token of each of `batch` sessions: row b is the query of the newest
+ * position lens[b] - 1 of slot slots[b] (slots null: slot b), whose cache
+ * starts at element slots[b] * slot_stride. lens and slots are device int32;
+ * 0 <= lens[b] <= max_len <= ctx, where max_len is the host's bound that sizes
+ * the launch. lens[b] == 0 gives a row of zeros. acc [n_slots][kv_heads][ctx]
+ * fp32 (may be null): the attention weight that each seen position got is
+ * added to it, summed over the query heads of the KV head; the slots are then
+ * distinct. A slot or a length out of range gives a row of zeros and is
+ * reported by lfm_attention_status. batch <= 65535. */
+lfm_status lfm_attention_decode(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* k_cache,
+                                const void* v_cache, uint64_t slot_stride, uint32_t n_slots, const int32_t* slots,
+                                const int32_t* lens, uint32_t batch, uint32_t max_len, uint32_t window,
+                                uint32_t sinks, float* acc, void* out, uint64_t out_stride, void* stream);
+
+/* One token of each of `batch` sessions that share a prefix: row b sees the
+ * prefix_len positions of the prefix cache [kv_heads][prefix_ctx][head_dim]
+ * and the lens[b] positions of its own slot (as in lfm_attention_decode,
+ * lens[b] may be 0; with prefix_len 0 too the row is zeros). The prefix is
+ * read once for all sessions, not once for each. `workspace` (16-byte aligned) has at least
+ * lfm_attention_shared_workspace bytes; calls that overlap on the GPU, and
+ * captured graphs that may, have one each. */
+size_t lfm_attention_shared_workspace(const lfm_attn_shape* shape, uint32_t batch, uint32_t prefix_len);
+lfm_status lfm_attention_shared(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* prefix_k,
+                                const void* prefix_v, uint32_t prefix_ctx, uint32_t prefix_len, const void* k_cache,
+                                const void* v_cache, uint64_t slot_stride, uint32_t n_slots, const int32_t* slots,
+                                const int32_t* lens, uint32_t batch, uint32_t max_len, void* out,
+                                uint64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The attention weights of a prompt, summed per cache position: acc[kv][j] +=
+ * sum over the queries t and the query heads h of KV head kv of
+ * exp(scale q_th.k_j - lse[t][h]), for the positions that t sees. acc
+ * [kv_heads][ctx] fp32 is one slot's; lse is that of lfm_attention_window for
+ * the same queries. All n queries may be given, or only the last few
+ * that should choose what the cache keeps. The sums come out the same on every run. */
+lfm_status lfm_attention_weights(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* k_cache,
+                                 uint32_t start, uint32_t n, uint32_t window, uint32_t sinks, const float* lse,
+                                 float* acc, void* stream);
+
+/* Eviction: of each session b with lens[b] > budget, every KV head keeps its
+ * first keep_first positions, its last keep_last and, of the rest, those with
+ * the largest acc (equal: the earlier position; NaN ranks below every number)
+ * until budget are kept; keep_first + keep_last <= budget. What is kept moves
+ * to the front in its old order: K and V rows, acc and pos ([n_slots]
+ * [kv_heads][ctx] int32, the caller's record of what a cache row holds; may be
+ * null), from the source arrays to the same slots of the destination arrays,
+ * which are the source arrays themselves (in place; all of them then) or do
+ * not overlap them. lens_out[b] = min(lens[b], budget), in another array than
+ * lens. Rows behind the kept ones are left as they were. Only dtype's cache type, kv_heads, head_dim and
+ * ctx of `shape` are used. Slots are distinct: a session whose slot an earlier
+ * one has, or whose slot or length is out of range, is left out and reported
+ * by lfm_attention_status. batch <= 65535. */
+lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const void* v_src, const float* acc_src,
+                           const int32_t* pos_src, void* k_dst, void* v_dst, float* acc_dst, int32_t* pos_dst,
+                           uint64_t slot_stride, uint32_t n_slots, const int32_t* slots, const int32_t* lens,
+                           int32_t* lens_out, uint32_t batch, uint32_t max_len, uint32_t budget, uint32_t keep_first,
+                           uint32_t keep_last, void* stream);
+
+/* Waits for `stream` and returns what the calls above have reported on the
+ * current device since the last call of this one, as the sum of LFM_ATTN_BAD_*;
+ * 0: nothing. A device-side wait that ran out (about a second) reports
+ * LFM_ATTN_BAD_WAIT; the results of the calls since then are not to be used. */
+#define LFM_ATTN_BAD_WAIT 1u
+#define LFM_ATTN_BAD_SLOT 2u
+#define LFM_ATTN_BAD_LEN 4u
+lfm_status lfm_attention_status(uint32_t* status, void* stream);
+
 /* Tensor-core (tcgen05 / TMEM) Q6_K prompt GEMM, the prefill counterpart of
  * lfm_q6k_matmul with the same contract: y[o + j*rows] = sum_k W[o,k]
  * x[k + j*in_dim] for n columns (q6k_prompt, ops.rs:340-374). Weights enter

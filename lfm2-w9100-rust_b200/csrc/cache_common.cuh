@@ -1,0 +1,70 @@
+// Device helpers of the session-cache attention kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "cache_attn.h"
+#include "dev_common.cuh"
+
+namespace lfm {
+namespace cache {
+
+// What the kernels of the including file report. The kernels name the variable
+// itself, so that a launch needs no address from the host.
+static __device__ unsigned g_status;
+__device__ __forceinline__ void report(unsigned bits) { atomicOr(&g_status, bits); }
+
+inline cudaError_t take_status(unsigned* bits, cudaStream_t s) {
+  unsigned *at = nullptr, got = 0;
+  cudaError_t e = cudaGetSymbolAddress((void**)&at, g_status);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&got, at, sizeof got, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof got, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  *bits |= got;
+  return e;
+}
+
+// The element types of LFM_ATTN_*: q and out, and the caches.
+template <int T>
+struct Types;
+template <>
+struct Types<T_F32> {
+  using Q = float;
+  using C = __half;
+};
+template <>
+struct Types<T_F16> {
+  using Q = __half;
+  using C = __half;
+};
+template <>
+struct Types<T_BF16> {
+  using Q = __nv_bfloat16;
+  using C = __nv_bfloat16;
+};
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
+__device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
+__device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
+
+// The slot and the length of session b, checked: false leaves the session out.
+__device__ __forceinline__ bool session(const int* slots, const int* lens, int b, int n_slots, int most, int* slot,
+                                        int* len) {
+  *slot = slots ? slots[b] : b;
+  *len = lens[b];
+  const unsigned bad = ((unsigned)*slot >= (unsigned)n_slots ? BAD_SLOT : 0u) |
+                       ((unsigned)*len > (unsigned)most ? BAD_LEN : 0u);
+  if (bad && threadIdx.x == 0) report(bad);
+  return !bad;
+}
+
+// First position of the window of a query at position p (0: no window).
+__host__ __device__ __forceinline__ int window_first(int p, int window) {
+  return window > 0 && window <= p ? p - window + 1 : 0;
+}
+
+}  // namespace cache
+}  // namespace lfm

@@ -34,6 +34,9 @@ struct LaunchCfg {
   int sms = 148;
 };
 
+// Sets this thread's lfm_ops_error message (ops.cu).
+void ops_set_error(const char* message) noexcept;
+
 // ---------------------------------------------------------------- decode
 // y[r] = W x (q6k_matmul, kernels.rs:832-1025, n == 1)
 void mv_plain(const Q6Mat& W, XSrc xs, float* y, const LaunchCfg& c);

@@ -46,6 +46,16 @@ __global__ void k_selftest_wait_timeout(unsigned* err, unsigned long long* cycle
 }
 }  // namespace
 
+namespace lfm {
+void ops_set_error(const char* message) noexcept {
+  try {
+    t_err = message;
+  } catch (...) {
+    t_err.clear();  // no memory for the message
+  }
+}
+}  // namespace lfm
+
 extern "C" {
 
 size_t lfm_q6k_device_bytes(uint32_t in_dim, uint32_t rows) {

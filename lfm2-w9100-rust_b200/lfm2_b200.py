@@ -39,6 +39,13 @@ class Counters(ctypes.Structure):
                  "expert_grouped_launches")]
 
 
+class AttnShape(ctypes.Structure):
+    """lfm_attn_shape: element types (0: fp32 q and out over fp16 caches, 1: fp16, 2: bf16), head layout and
+    positions of a cache slot; scale 0 is 1/sqrt(head_dim)."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("dtype", "heads", "kv_heads", "head_dim", "ctx")] + \
+               [("scale", ctypes.c_float)]
+
+
 _lib = None
 
 # Every symbol declared in include/lfm_cuda.h.
@@ -54,6 +61,8 @@ EXPORTS = [
     "lfm_q6k_upload", "lfm_q6k_dequant", "lfm_q6k_matmul", "lfm_q6k_routed", "lfm_route",
     "lfm_argmax", "lfm_argmax_noalloc", "lfm_tc_gemm_f16", "lfm_tc_gemm_f16_bmn", "lfm_attention_prefill", "lfm_selftest_wait_timeout", "lfm_q6k_prompt_gemm", "lfm_q6k_prompt_grouped",
     "lfm_q6k_expand_f16", "lfm_q6k_prompt_gemm_x16", "lfm_q6k_prompt_grouped_x16",
+    "lfm_attention_window", "lfm_attention_decode", "lfm_attention_shared_workspace", "lfm_attention_shared",
+    "lfm_attention_weights", "lfm_cache_evict", "lfm_attention_status",
     "lfm_ops_error",
     "lfm_text_create", "lfm_text_destroy", "lfm_text_push", "lfm_text_finish", "lfm_text_reset", "lfm_text_error",
 ]
@@ -68,6 +77,7 @@ def lib() -> ctypes.CDLL:
         raise LfmError(f"{LIB_PATH} is missing: run lfm2-w9100-rust_b200/build.py (no CPU fallback)")
     L = ctypes.CDLL(LIB_PATH)
     P, U32, I64, SZ = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_int64, ctypes.c_size_t
+    U64, S = ctypes.c_uint64, ctypes.POINTER(AttnShape)
     st = ctypes.c_int32
     sig = {
         "lfm_model_inspect": ([ctypes.c_char_p, ctypes.POINTER(Hparams)], st),
@@ -117,6 +127,13 @@ def lib() -> ctypes.CDLL:
         "lfm_q6k_expand_f16": ([P, U32, U32, P, P], st),
         "lfm_q6k_prompt_gemm_x16": ([P, P, U32, U32, P, U32, P, P], st),
         "lfm_q6k_prompt_grouped_x16": ([P, P, U32, U32, U32, P, P, U32, U32, P, P], st),
+        "lfm_attention_window": ([S, P, U64, P, P, U32, U32, U32, U32, P, U64, P, P], st),
+        "lfm_attention_decode": ([S, P, U64, P, P, U64, U32, P, P, U32, U32, U32, U32, P, P, U64, P], st),
+        "lfm_attention_shared_workspace": ([S, U32, U32], SZ),
+        "lfm_attention_shared": ([S, P, U64, P, P, U32, U32, P, P, U64, U32, P, P, U32, U32, P, U64, P, SZ, P], st),
+        "lfm_attention_weights": ([S, P, U64, P, U32, U32, U32, U32, P, P, P], st),
+        "lfm_cache_evict": ([S, P, P, P, P, P, P, P, P, U64, U32, P, P, P, U32, U32, U32, U32, U32, P], st),
+        "lfm_attention_status": ([ctypes.POINTER(U32), P], st),
         "lfm_ops_error": ([], ctypes.c_char_p),
         "lfm_text_create": ([P, P, U32, U32, ctypes.c_int, ctypes.c_int, ctypes.POINTER(P)], st),
         "lfm_text_destroy": ([P], None),

@@ -16,6 +16,13 @@ pub const LFM_ERR_STATE: lfm_status = 4;
 pub const LFM_ERR_DEVICE: lfm_status = 5;
 pub const LFM_MAX_CTX: u32 = 4096;
 pub const LFM_PREFILL_CHUNK: u32 = 64;
+pub const LFM_ATTN_F32: u32 = 0;
+pub const LFM_ATTN_F16: u32 = 1;
+pub const LFM_ATTN_BF16: u32 = 2;
+pub const LFM_ATTN_MAX_GROUP: u32 = 8;
+pub const LFM_ATTN_BAD_WAIT: u32 = 1;
+pub const LFM_ATTN_BAD_SLOT: u32 = 2;
+pub const LFM_ATTN_BAD_LEN: u32 = 4;
 pub const LFM_EP_OWN_SESSION: u32 = 0xFFFF_FFFF;
 
 /// Opaque engine handle.
@@ -49,6 +56,18 @@ pub struct lfm_hparams {
     pub eps: f32,
     pub rope_theta: f32,
     pub kv_heads: [u32; 64],
+}
+
+/// `lfm_attn_shape`: types and head layout of the session-cache attention calls.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct lfm_attn_shape {
+    pub dtype: u32,
+    pub heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub ctx: u32,
+    pub scale: f32,
 }
 
 /// `lfm_counters` (the counters of main.rs:273-280 and persistent.rs:230-242).
@@ -129,6 +148,31 @@ extern "C" {
     pub fn lfm_attention_prefill(q_dev: *const f32, q_stride: u32, k_cache: *const c_void, v_cache: *const c_void,
                                  ctx: u32, start: u32, n: u32, out_dev: *mut f32, out_stride: u32,
                                  stream: *mut c_void) -> lfm_status;
+    pub fn lfm_attention_window(shape: *const lfm_attn_shape, q: *const c_void, q_stride: u64,
+                                k_cache: *const c_void, v_cache: *const c_void, start: u32, n: u32, window: u32,
+                                sinks: u32, out: *mut c_void, out_stride: u64, lse: *mut f32,
+                                stream: *mut c_void) -> lfm_status;
+    pub fn lfm_attention_decode(shape: *const lfm_attn_shape, q: *const c_void, q_stride: u64,
+                                k_cache: *const c_void, v_cache: *const c_void, slot_stride: u64, n_slots: u32,
+                                slots: *const i32, lens: *const i32, batch: u32, max_len: u32, window: u32,
+                                sinks: u32, acc: *mut f32, out: *mut c_void, out_stride: u64,
+                                stream: *mut c_void) -> lfm_status;
+    pub fn lfm_attention_shared_workspace(shape: *const lfm_attn_shape, batch: u32, prefix_len: u32) -> usize;
+    pub fn lfm_attention_shared(shape: *const lfm_attn_shape, q: *const c_void, q_stride: u64,
+                                prefix_k: *const c_void, prefix_v: *const c_void, prefix_ctx: u32, prefix_len: u32,
+                                k_cache: *const c_void, v_cache: *const c_void, slot_stride: u64, n_slots: u32,
+                                slots: *const i32, lens: *const i32, batch: u32, max_len: u32, out: *mut c_void,
+                                out_stride: u64, workspace: *mut c_void, workspace_bytes: usize,
+                                stream: *mut c_void) -> lfm_status;
+    pub fn lfm_attention_weights(shape: *const lfm_attn_shape, q: *const c_void, q_stride: u64,
+                                 k_cache: *const c_void, start: u32, n: u32, window: u32, sinks: u32,
+                                 lse: *const f32, acc: *mut f32, stream: *mut c_void) -> lfm_status;
+    pub fn lfm_cache_evict(shape: *const lfm_attn_shape, k_src: *const c_void, v_src: *const c_void,
+                           acc_src: *const f32, pos_src: *const i32, k_dst: *mut c_void, v_dst: *mut c_void,
+                           acc_dst: *mut f32, pos_dst: *mut i32, slot_stride: u64, n_slots: u32, slots: *const i32,
+                           lens: *const i32, lens_out: *mut i32, batch: u32, max_len: u32, budget: u32,
+                           keep_first: u32, keep_last: u32, stream: *mut c_void) -> lfm_status;
+    pub fn lfm_attention_status(status: *mut u32, stream: *mut c_void) -> lfm_status;
     pub fn lfm_q6k_prompt_gemm(w_dev: *const c_void, in_dim: u32, rows: u32, x_dev: *const f32, n: u32,
                                y_dev: *mut f32, stream: *mut c_void) -> lfm_status;
     pub fn lfm_q6k_prompt_grouped(w_dev: *const c_void, in_dim: u32, rows: u32, n_expert: u32,
