@@ -192,7 +192,7 @@ cudaError_t weights(const Prompt& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t decode(const Decode& a, cudaStream_t s) {
+cudaError_t shared(const Decode& a, cudaStream_t s) {
   by_type(a.type, a.d, [&](auto t, auto d) {
     k_decode<decltype(t)::value, decltype(d)::value><<<dim3(a.kv_heads, a.batch), 32 * (a.heads / a.kv_heads), 0, s>>>(a);
   });
@@ -202,8 +202,6 @@ cudaError_t decode(const Decode& a, cudaStream_t s) {
 cudaError_t take_status_attn(unsigned* bits, cudaStream_t s) { return take_status(bits, s); }
 
 size_t shared_workspace(const Decode&) { return 16; }
-
-cudaError_t shared(const Decode& a, cudaStream_t s) { return decode(a, s); }
 
 }  // namespace cache
 }  // namespace lfm

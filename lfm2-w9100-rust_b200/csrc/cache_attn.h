@@ -69,6 +69,7 @@ cudaError_t shared(const Decode& a, cudaStream_t s);
 cudaError_t evict(const Evict& a, cudaStream_t s);
 // Adds what the kernels of each file have reported on this device to *bits and clears it; waits for the stream.
 cudaError_t take_status_attn(unsigned* bits, cudaStream_t s);
+cudaError_t take_status_decode(unsigned* bits, cudaStream_t s);
 cudaError_t take_status_evict(unsigned* bits, cudaStream_t s);
 
 }  // namespace cache

@@ -169,6 +169,7 @@ DECODE = [  # kind, heads, kv, d, ctx, lens, window, sinks, acc, pad
     ("bf16", 32, 4, 128, 1100, [1100, 3, 0, 999], 128, 5, True, 0),
     ("bf16", 7, 7, 64, 90, [90, 89, 5], 50, 60, False, 8),
     ("bf16", 8, 1, 128, 9000, [9000], 0, 0, True, 0),
+    ("f16", 8, 1, 64, 60000, [60000, 0, 53], 0, 0, True, 0),
 ]
 
 
