@@ -64,11 +64,13 @@ struct Evict {
 cudaError_t window(const Prompt& a, cudaStream_t s);
 cudaError_t weights(const Prompt& a, cudaStream_t s);
 cudaError_t decode(const Decode& a, cudaStream_t s);
+// decode joined with the prefix's part: o [kv head][session * g + head][d] not divided by l, ml (m in log2 units, l)
+cudaError_t decode_joined(const Decode& a, const float* o, const float2* ml, cudaStream_t s);
 size_t shared_workspace(const Decode& a);
 cudaError_t shared(const Decode& a, cudaStream_t s);
 cudaError_t evict(const Evict& a, cudaStream_t s);
 // Adds what the kernels of each file have reported on this device to *bits and clears it; waits for the stream.
-cudaError_t take_status_attn(unsigned* bits, cudaStream_t s);
+cudaError_t take_status_tc(unsigned* bits, cudaStream_t s);
 cudaError_t take_status_decode(unsigned* bits, cudaStream_t s);
 cudaError_t take_status_evict(unsigned* bits, cudaStream_t s);
 

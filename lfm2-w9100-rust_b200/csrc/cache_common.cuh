@@ -50,6 +50,48 @@ __device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
 __device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(dev::smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_peer(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_peer4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+
+// 2^x by the hardware's instruction, within 2^-22 of it; results under 2^-126 are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 32 accumulators times `by`, as 32 neighbouring outputs at 16-byte aligned dst.
+template <class Q>
+__device__ __forceinline__ void store_row(Q* dst, const uint32_t (&v)[32], float by) {
+  constexpr int PER = 16 / sizeof(Q);
+#pragma unroll
+  for (int e = 0; e < 32; e += PER) {
+    __align__(16) Q x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) from_f32(__uint_as_float(v[e + i]) * by, &x[i]);
+    *(uint4*)(dst + e) = *(const uint4*)x;
+  }
+}
+
 // The slot and the length of session b, checked: false leaves the session out.
 __device__ __forceinline__ bool session(const int* slots, const int* lens, int b, int n_slots, int most, int* slot,
                                         int* len) {

@@ -57,35 +57,12 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float ld_peer(uint32_t at) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_peer4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at)
-               : "memory");
-  return v;
-}
-
 // The weight of a part whose maximum is m under the joint maximum M (no part: 0).
 __device__ __forceinline__ float part_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2f(m - M); }
 
 struct Joint {
-  const float* o;   // prefix partials [split][kv head][row][D], log2 units, not divided by l
-  const float2* ml; // their (m, l) [split][kv head][row]
-  int splits;
+  const float* o;    // the prefix's part [kv head][row][D], not divided by l; null: none
+  const float2* ml;  // its (m in log2 units, l) [kv head][row]
 };
 
 template <int T, int D, int ACC>
@@ -98,7 +75,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
   float* scores = (float*)(smem + RING);  // STORED: [head][cap]
   __shared__ uint64_t full[WARPS][STAGES];
   __shared__ __align__(16) float s_o[8][D];
-  __shared__ float s_m[8], s_l[8], w_m[WARPS][8], w_l[WARPS][8], f_m[8], f_inv[8];
+  __shared__ float s_m[8], s_l[8], w_m[WARPS][8], w_l[WARPS][8], f_m[8], f_inv[8], f_pre[8];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
   const int g = a.heads / a.kv_heads;
@@ -226,7 +203,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
     uint32_t p[TILES][2];  // [tile][hi, lo]
 #pragma unroll
     for (int kt = 0; kt < TILES; kt++) {
-      const float x = exp2f(s[kt][0] - m), y = exp2f(s[kt][1] - m);
+      const float x = exp2_fast(s[kt][0] - m), y = exp2_fast(s[kt][1] - m);
       l += x + y;
       if constexpr (std::is_same<C, __half>::value) {
         const __half2 h = __floats2half2_rn(x, y);
@@ -319,19 +296,18 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
     __syncthreads();
 
   // join the CTAs and the prefix's parts: the joint statistics of each head, then this CTA's share of the columns
-  if (pre.splits) pdl_wait();
-  const size_t rows = (size_t)a.batch * g;
+  if (pre.o) pdl_wait();
+  const size_t row0 = ((size_t)kh * a.batch + b) * g;  // of the prefix's part
   if (tid < g) {
     float M = -INFINITY, L = 0.f;
     for (int x = 0; x < nranks; x++) M = fmaxf(M, ld_peer(peer(&s_m[tid], x)));
-    for (int x = 0; x < pre.splits; x++)
-      M = fmaxf(M, pre.ml[((size_t)x * a.kv_heads + kh) * rows + (size_t)b * g + tid].x);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (pre.o) ml = pre.ml[row0 + tid];
+    M = fmaxf(M, ml.x);
     for (int x = 0; x < nranks; x++)
       L = fmaf(part_weight(ld_peer(peer(&s_m[tid], x)), M), ld_peer(peer(&s_l[tid], x)), L);
-    for (int x = 0; x < pre.splits; x++) {
-      const float2 ml = pre.ml[((size_t)x * a.kv_heads + kh) * rows + (size_t)b * g + tid];
-      L = fmaf(part_weight(ml.x, M), ml.y, L);
-    }
+    L = fmaf(part_weight(ml.x, M), ml.y, L);
+    f_pre[tid] = part_weight(ml.x, M);
     f_m[tid] = M;
     f_inv[tid] = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing seen: zeros
   }
@@ -346,10 +322,9 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
       const float4 y = ld_peer4(peer(&s_o[h][c], x));
       f.x = fmaf(wt, y.x, f.x), f.y = fmaf(wt, y.y, f.y), f.z = fmaf(wt, y.z, f.z), f.w = fmaf(wt, y.w, f.w);
     }
-    for (int x = 0; x < pre.splits; x++) {
-      const size_t row = ((size_t)x * a.kv_heads + kh) * rows + (size_t)b * g + h;
-      const float wt = part_weight(pre.ml[row].x, M);
-      const float4 y = *(const float4*)(pre.o + row * D + c);
+    if (pre.o) {
+      const float wt = f_pre[h];
+      const float4 y = *(const float4*)(pre.o + (row0 + h) * D + c);
       f.x = fmaf(wt, y.x, f.x), f.y = fmaf(wt, y.y, f.y), f.z = fmaf(wt, y.z, f.z), f.w = fmaf(wt, y.w, f.w);
     }
     Q* dst = (Q*)a.out + (size_t)b * a.out_stride + (size_t)(kh * g + h) * D + c;
@@ -365,7 +340,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
       if constexpr (ACC == STORED) {
         for (int i = tid; i < count; i += WARPS * 32) {
           float sum = 0.f;
-          for (int h = 0; h < g; h++) sum = fmaf(exp2f(scores[h * cap + i] - f_m[h]), f_inv[h], sum);
+          for (int h = 0; h < g; h++) sum = fmaf(exp2_fast(scores[h * cap + i] - f_m[h]), f_inv[h], sum);
           const int j = first + i;
           atomicAdd(acc + (j < hi ? j : lo + j - hi), sum);
         }
@@ -385,7 +360,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
           for (int kt = 0; kt < TILES; kt++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float x = exp2f(s[kt][e] - M) * inv;
+              float x = exp2_fast(s[kt][e] - M) * inv;
               x += __shfl_xor_sync(0xffffffffu, x, 4);
               x += __shfl_xor_sync(0xffffffffu, x, 8);
               x += __shfl_xor_sync(0xffffffffu, x, 16);
@@ -423,7 +398,7 @@ cudaError_t launch(const Decode& a, const Joint& pre, int nranks, int cap, cudaS
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   c.attrs = at;
-  c.numAttrs = pre.splits ? 2 : 1;
+  c.numAttrs = pre.o ? 2 : 1;
   return cudaLaunchKernelEx(&c, f, a, pre, cap);
 }
 
@@ -451,10 +426,10 @@ cudaError_t run(const Decode& a, const Joint& pre, cudaStream_t s) {
 }
 }  // namespace
 
-cudaError_t decode(const Decode& a, cudaStream_t s) { return run(a, Joint{nullptr, nullptr, 0}, s); }
+cudaError_t decode(const Decode& a, cudaStream_t s) { return run(a, Joint{nullptr, nullptr}, s); }
 
-cudaError_t decode_joined(const Decode& a, const float* o, const float2* ml, int splits, cudaStream_t s) {
-  return run(a, Joint{o, ml, splits}, s);
+cudaError_t decode_joined(const Decode& a, const float* o, const float2* ml, cudaStream_t s) {
+  return run(a, Joint{o, ml}, s);
 }
 
 cudaError_t take_status_decode(unsigned* bits, cudaStream_t s) { return take_status(bits, s); }

@@ -230,7 +230,7 @@ lfm_status lfm_attention_status(uint32_t* status, void* stream) {
   const char* who = "lfm_attention_status";
   if (!status) return bad(who, "status is null");
   unsigned bits = 0;
-  cudaError_t e = lfm::cache::take_status_attn(&bits, (cudaStream_t)stream);
+  cudaError_t e = lfm::cache::take_status_tc(&bits, (cudaStream_t)stream);
   if (e == cudaSuccess) e = lfm::cache::take_status_decode(&bits, (cudaStream_t)stream);
   if (e == cudaSuccess) e = lfm::cache::take_status_evict(&bits, (cudaStream_t)stream);
   *status = bits;
