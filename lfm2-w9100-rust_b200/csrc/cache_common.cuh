@@ -79,6 +79,42 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t two(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 one(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Four neighbouring outputs.
+__device__ __forceinline__ void store4(float* dst, float4 v) { *(float4*)dst = v; }
+template <class H>
+__device__ __forceinline__ void store4(H* dst, float4 v) {
+  __align__(8) H x[4];
+  from_f32(v.x, x), from_f32(v.y, x + 1), from_f32(v.z, x + 2), from_f32(v.w, x + 3);
+  *(uint2*)dst = *(const uint2*)x;
+}
+
 // 32 accumulators times `by`, as 32 neighbouring outputs at 16-byte aligned dst.
 template <class Q>
 __device__ __forceinline__ void store_row(Q* dst, const uint32_t (&v)[32], float by) {

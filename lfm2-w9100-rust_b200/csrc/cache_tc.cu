@@ -6,18 +6,25 @@
 // Rows are packed: row R of a KV head is query head R % g of token (or session)
 // R / g, so every group size fills the 128-row tiles. A CTA holds two tiles of
 // rows and walks the positions in tiles of 128, with
-//   warp 0      TMA: K and V tiles into one ring of slots
-//   warp 1      TMEM and the MMAs: S_x = Q_x K^T, O_x += P_x V for tile x
-//   warps 4-7   the softmax of tile 0, warps 8-11 that of tile 1: one thread a row
-// While one tile is in its softmax, the products of the other run. The weights
-// P take the place of S in tensor memory (a 16-bit operand of half its width)
-// and enter the second product from there. For fp32 queries q and P are fp16
-// hi/lo pairs, two MMAs each; the pair of weights fills the whole of S.
-// O stays in tensor memory; a row's maximum is raised, and O rescaled, only
-// when it grows by more than 2^8, which keeps every weight inside fp16's range
-// and every rounding relative.
+//   warp 0       TMA: K and V tiles into one ring of slots
+//   warp 1       TMEM and the MMAs: S_x = Q_x K^T, O_x += P_x V for tile x
+//   warps 2-9    the softmax of tile 0, warps 10-17 that of tile 1
+// While one tile is in its softmax, the products of the other run. A row is
+// shared by two threads, one for each half of its columns, which exchange
+// maxima through shared memory: with four softmax warps to a scheduler their
+// latencies overlap (one thread a row took 2.4 times as long: 311 us for 8192 bf16
+// tokens under a window of 1500). The weights P take the place of S in tensor
+// memory and enter the second product from there.
+//
+// 16-bit queries: O stays in tensor memory, and a row's maximum is raised, and O
+// rescaled, only when it grows by more than 2^8, which keeps every weight inside
+// fp16's range and every rounding relative. fp32 queries: q and P are fp16 hi/lo
+// pairs, two MMAs each, the low parts first; the tensor core cuts its sums off
+// instead of rounding them, a loss that grows with their number (2.2e-6 over
+// 1024 positions), so O of each tile starts from zero and is added to the
+// running output in registers.
 // Few row blocks leave SMs idle, so a cluster of CTAs may split the positions of
-// one block and join through distributed shared memory.
+// one block; each sends its part of a row to the CTA that finishes the row.
 // Every wait is bounded; one that runs out is reported and the CTA releases
 // its tensor memory.
 #include <cuda.h>
@@ -37,13 +44,10 @@ namespace {
 using namespace dev;
 using namespace tc;
 
-constexpr int THREADS = 384, KT = 128, ROWS = 256;
+constexpr int THREADS = 576, KT = 128, ROWS = 256;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-// Registers of a thread: at launch, after the split between the two kinds of warps.
-constexpr int REGS = 168, REGS_ISSUE = 72, REGS_SOFTMAX = 216;
-static_assert(128 * REGS_ISSUE + 256 * REGS_SOFTMAX <= THREADS * REGS, "the split asks for more than the launch has");
 constexpr float GROWTH = 8.f;  // log2 of what a row may grow before its maximum is raised
-constexpr uint32_t COLS = 512, COL_O = 256;  // S_x: [128 x, 128 x + 128); O_x: [256 + D x, + D)
+constexpr uint32_t COLS = 512, COL_O = 256;  // S_x: [128 x, 128 x + 128); the O buffers from 256 on, D each
 
 template <int T, int D>
 struct Cfg {
@@ -51,10 +55,16 @@ struct Cfg {
   static constexpr int CHUNK = 128 * 128;             // 128 rows x 64 16-bit values, swizzled
   static constexpr int TILE = CHUNK * (D / 64);       // 128 rows x D
   static constexpr int Q_BYTES = 2 * (PAIR ? 2 : 1) * TILE;
-  static constexpr int SLOTS = std::min(6, (226 * 1024 - Q_BYTES) / TILE);
-  static constexpr int SMEM = Q_BYTES + SLOTS * TILE + 1024;
+  // buffers of the maxima that two threads exchange; one costs a second barrier and is taken where memory is short
+  static constexpr int MAXIMA = PAIR && D == 128 ? 1 : 2;
+  static constexpr int STATIC = MAXIMA == 1 ? 3072 : 5120;
+  static constexpr int SLOTS = std::min(6, (227 * 1024 - STATIC - Q_BYTES) / TILE);
+  static constexpr int SMEM = Q_BYTES + SLOTS * TILE;
+  // O buffers of a row tile: fp32 queries fold one while the next product fills the other, where there is room
+  static constexpr int OBUF = PAIR && D == 64 ? 2 : 1;
   static constexpr int STRIDE = D + 4;  // floats of a row in the join: rows of one column start in different banks
-  static_assert(SLOTS >= 3 && ROWS * (STRIDE * 4 + 8) <= Q_BYTES + SLOTS * TILE, "shared memory");
+  static_assert(SLOTS >= 3 && 512 - COL_O >= 2 * OBUF * D, "memories");
+  static_assert(ROWS * (STRIDE * 4 + 8) <= Q_BYTES + SLOTS * TILE, "the join takes the place of queries and ring");
 };
 
 struct Rows {
@@ -138,11 +148,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   using C = typename Types<T>::C;
   constexpr bool PAIR = F::PAIR;
   constexpr uint32_t BF = std::is_same<C, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* slots = smem + F::Q_BYTES;
   __shared__ uint64_t q_full, full[F::SLOTS], empty[F::SLOTS], s_full[2], p_full[2];
   __shared__ uint32_t tmem_at;
+  __shared__ float s_max[F::MAXIMA][2][ROWS];  // [tile parity][half][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
   const int r0 = (int)(gridDim.z - 1 - blockIdx.z) * ROWS;  // the longest rows first
@@ -154,14 +164,14 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int i0 = (int)((long long)tiles.n * rank / nranks), i1 = (int)((long long)tiles.n * (rank + 1) / nranks);
 
   if (tid == 0) {
-    mbar_init(&q_full, 8);
+    mbar_init(&q_full, 16);
     for (int i = 0; i < F::SLOTS; i++) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int x = 0; x < 2; x++) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);
+      mbar_init(&p_full[x], 8);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -171,10 +181,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_at;
   const int count = i1 - i0;
-  float2 ml = make_float2(-INFINITY, 0.f);  // this thread's row
+  if (nranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+  if (warp < 2) {
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
       int n = 0;
@@ -213,7 +222,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int kk = 0; kk < D / 16; kk++) {
               const uint32_t off = (kk >> 2) * F::CHUNK + (kk & 3) * 32;
-              mma_f16(d, smem_desc_sw128(qb + h * F::TILE + off), smem_desc_sw128(kb + off), idesc, h || kk);
+              mma_f16(d, smem_desc_sw128(qb + (PAIR ? 1 - h : 0) * F::TILE + off), smem_desc_sw128(kb + off), idesc,
+                      h || kk);
             }
         }
       };
@@ -232,10 +242,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         tc_fence_after();
         if (one) {
-          const uint32_t d = tmem + COL_O + D * x, p = tmem + 128 * x, v = smem_u32(vb);
-          for (int h = 0; h < (PAIR ? 2 : 1); h++)
+          const uint32_t d = tmem + COL_O + D * (F::OBUF * x + ((i - i0) & (F::OBUF - 1)));
+          const uint32_t p = tmem + 128 * x, v = smem_u32(vb);
+          for (int h = 0; h < (PAIR ? 2 : 1); h++)  // 32 columns of S hold 16 columns of weights, and behind them their low parts
             for (int kk = 0; kk < width / 16; kk++)
-              mma_ts(d, p + 64 * h + 8 * kk, smem_desc_mn_sw128(v + kk * 2048, F::CHUNK), IDESC_PV, i > i0 || h || kk);
+              mma_ts(d, p + 32 * (kk >> 1) + 8 * (kk & 1) + (PAIR && h == 0 ? 16 : 0),
+                     smem_desc_mn_sw128(v + kk * 2048, F::CHUNK), IDESC_PV, (!PAIR && i > i0) || h || kk);
         }
       };
       for (int x = 0; x < ntiles_x; x++) {
@@ -261,15 +273,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-    const int x = (warp - 4) >> 2, quarter = warp & 3, rt = quarter * 32 + lane, row = x * 128 + rt;
+    const int x = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1, quarter = warp & 3;  // TMEM lanes by warp % 4
+    const int rt = quarter * 32 + lane, row = x * 128 + rt;
     const int R = r0 + min(row, nrows - 1), tok = R / a.g, head = kh * a.g + R % a.g;
     const bool live = row < nrows;
     {
       const Q* q = (const Q*)a.q + (size_t)tok * a.q_stride + (size_t)head * D;
       uint8_t* dst = smem + x * (F::Q_BYTES / 2);
 #pragma unroll
-      for (int c = 0; c < D / 8; c++) {
+      for (int i = 0; i < D / 16; i++) {
+        const int c = half * (D / 16) + i;
         uint8_t* chunk = dst + (c >> 3) * F::CHUNK;
         if constexpr (PAIR) {
           const float4 u = *(const float4*)(q + 8 * c), v = *(const float4*)(q + 8 * c + 4);
@@ -292,53 +305,73 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) mbar_arrive(&q_full);
     }
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t sbase = mine + 128 * x, obase = mine + COL_O + D * x;
+    const uint32_t sbase = mine + 128 * x + 64 * half, obase = mine + COL_O + D * F::OBUF * x + (D / 2) * half;
     const float sc = PAIR ? 1.f : a.scale2;
     const int p = a.start + tok;
     const int wlo = a.window > 0 ? p - a.window + 1 : -0x40000000;
-    float m = -INFINITY, l = 0.f;
+    const int pair = 1 + 4 * x + quarter;  // the named barrier of the two warps that share these rows
+    float m = -INFINITY, l = 0.f, alpha_last = 0.f;
+    float o[PAIR ? D / 2 : 1] = {};  // fp32 queries: this half's columns of the running output
     bool ok = true;
+    auto fold = [&](int n) {  // O of the n-th tile, whose maximum came with alpha_last
+      if constexpr (PAIR) {
+#pragma unroll
+        for (int c = 0; c < D / 32; c++) {
+          uint32_t v[16];
+          tmem_ld16_nowait(obase + D * (n & (F::OBUF - 1)) + 16 * c, v);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[16 * c + e] = fmaf(o[16 * c + e], alpha_last, __uint_as_float(v[e]));
+        }
+      }
+    };
     if (x < ntiles_x) {
       for (int i = i0; i < i1; i++) {
-        if (!(ok = mbar_wait(&s_full[x], (i - i0) & 1, nullptr))) break;
+        const int n = i - i0;
+        if (ok) ok = mbar_wait(&s_full[x], n & 1, nullptr);  // a warp that gave up still meets its partner below
         tc_fence_after();
-        const int j0 = tiles.first(i), width = tiles.width(i), valid = tiles.valid(i);
-        uint32_t s[KT];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t v[32];
-          if (32 * c < width) {
-            tmem_ld32_nowait(sbase + 32 * c, v);
-#pragma unroll
-            for (int e = 0; e < 32; e++) s[32 * c + e] = v[e];
-          }
-        }
-        tmem_wait_ld();
-        // the tile is masked for some row of the block, or ends early
+        const int j0 = tiles.first(i) + 64 * half, width = tiles.width(i) - 64 * half, valid = tiles.valid(i) - 64 * half;
+        // the columns that some row of the block does not see
         const bool full_tile =
-            valid == KT && (a.prefix || i < tiles.ns ||
-                            (j0 + KT - 1 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + KT <= a.sinks)));
-        if (!full_tile) {
-          int cmax = valid - 1, cmin = -1, csink = 0;
-          if (!a.prefix && i >= tiles.ns) cmax = min(cmax, p - j0), cmin = wlo - j0, csink = a.sinks - j0;
+            valid >= 64 && (a.prefix || i < tiles.ns ||
+                            (j0 + 63 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + 64 <= a.sinks)));
+        int cmax = valid - 1, cmin = -1, csink = 0;
+        if (!a.prefix && i >= tiles.ns) cmax = min(cmax, p - j0), cmin = wlo - j0, csink = a.sinks - j0;
+        // S is read twice, for the maximum and for the weights: a thread's 64 columns do not fit beside the rest of
+        // its registers (292 bytes of spills for 16-bit queries)
+        auto take = [&](int c, uint32_t(&v)[32]) {
+          tmem_ld32(sbase + 32 * c, v);
+          if (!full_tile) {
 #pragma unroll
-          for (int e = 0; e < KT; e++)
-            if (!(e <= cmax && (e >= cmin || e < csink))) s[e] = 0xff800000u;
-        }
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-          if (32 * c < width) {
-#pragma unroll
-            for (int e = 0; e < 32; e++) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(s[32 * c + e]));
+            for (int e = 0; e < 32; e++)
+              if (!(32 * c + e <= cmax && (32 * c + e >= cmin || 32 * c + e < csink))) v[e] = 0xff800000u;
           }
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc;
-        if (__any_sync(0xffffffffu, mx > m + GROWTH)) {
-          const float mn = fmaxf(m, mx);
-          const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn);
-          if (i > i0) {
+        };
+        float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < D / 32; c++) {
+        for (int c = 0; c < 2; c++)
+          if (32 * c < width) {
+            uint32_t v[32];
+            take(c, v);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+              my = max3(my, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+            }
+          }
+        mx = fmaxf(mx, my);
+        float(&exchange)[2][ROWS] = s_max[n & (F::MAXIMA - 1)];
+        exchange[half][row] = mx;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+        mx = fmaxf(mx, exchange[half ^ 1][row]) * sc;
+        if (F::MAXIMA == 1) asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+        float alpha = 1.f;
+        if (PAIR || __any_sync(0xffffffffu, mx > m + GROWTH)) {
+          const float mn = fmaxf(m, mx);
+          alpha = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+          if (!PAIR && n > 0) {
+#pragma unroll
+            for (int c = 0; c < D / 64; c++) {
               uint32_t v[32];
               tmem_ld32(obase + 32 * c, v);
 #pragma unroll
@@ -349,120 +382,154 @@ __global__ void __launch_bounds__(THREADS, 1)
           l *= alpha;
           m = mn;
         }
+        if (F::OBUF == 1 && n > 0) fold(n - 1);
         const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: its weights are all 0
-        float l4[4] = {};
+        const uint64_t sc2 = two(sc, sc), ms2 = two(-ms, -ms);
+        uint64_t la = 0, lb = 0;  // pairs of 0.f
 #pragma unroll
-        for (int c = 0; c < 4; c++)
+        for (int c = 0; c < 2; c++)
           if (32 * c < width) {
-            uint32_t hi[16], lo[16];
+            uint32_t v[32], hi[16], lo[16];
+            take(c, v);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-              const float u = exp2_fast(fmaf(__uint_as_float(s[32 * c + 2 * e]), sc, -ms));
-              const float v = exp2_fast(fmaf(__uint_as_float(s[32 * c + 2 * e + 1]), sc, -ms));
-              l4[(2 * e) & 3] += u;
-              l4[(2 * e + 1) & 3] += v;
-              hi[e] = pack(C(), u, v);
-              if constexpr (PAIR) lo[e] = rest(hi[e], u, v);
+              const float2 z = one(fma2(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, ms2));
+              const float u = exp2_fast(z.x), w = exp2_fast(z.y);
+              if (e & 1)
+                lb = add2(lb, two(u, w));
+              else
+                la = add2(la, two(u, w));
+              hi[e] = pack(C(), u, w);
+              if constexpr (PAIR) lo[e] = rest(hi[e], u, w);
             }
-            tmem_st16(sbase + 16 * c, hi);
-            if constexpr (PAIR) tmem_st16(sbase + 64 + 16 * c, lo);
+            tmem_st16(sbase + 32 * c, hi);
+            if constexpr (PAIR) tmem_st16(sbase + 32 * c + 16, lo);
           }
-        l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+        const float2 sum = one(add2(la, lb));
+        l += sum.x + sum.y;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[x]);
+        if (F::OBUF == 2 && n > 0) fold(n - 1);
+        alpha_last = alpha;
       }
-      if (ok && count > 0) ok = mbar_wait(&s_full[x], count & 1, nullptr);  // the last product
-      tc_fence_after();
+      if (count > 0) {
+        if (ok) ok = mbar_wait(&s_full[x], count & 1, nullptr);  // the last product
+        tc_fence_after();
+        if (PAIR) fold(count - 1);
+      }
       if (!ok && lane == 0) report(BAD_WAIT);
     }
+    // ------------------------------------------------------------ epilogue
     const bool has = x < ntiles_x && count > 0;
-    if (has) ml = make_float2(m, l);
-    if (nranks == 1 && has) {
+    s_max[0][half][row] = l;
+    if (nranks == 1) {
+      asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+      l += s_max[0][half ^ 1][row];
       const float inv = l == 0.f && m == -INFINITY ? 0.f : 1.f / l;
       const size_t at = (size_t)kh * a.rows + R;
+      if (has) {
 #pragma unroll
-      for (int c = 0; c < D / 32; c++) {
-        uint32_t v[32];
-        __syncwarp();
-        tmem_ld32(obase + 32 * c, v);
-        if (live) {
-          if (a.prefix) {
+        for (int c = 0; c < D / 64; c++) {
+          uint32_t v[32];
+          __syncwarp();
+          if constexpr (PAIR) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = __float_as_uint(o[32 * c + e]);
+          } else {
+            tmem_ld32(obase + 32 * c, v);
+          }
+          const int col = (D / 2) * half + 32 * c;
+          if (live) {
+            if (a.prefix)
+              store_row<float>(a.part + at * D + col, v, 1.f);
+            else
+              store_row<Q>((Q*)a.out + (size_t)tok * a.out_stride + (size_t)head * D + col, v, inv);
+          }
+        }
+        if (live && half == 0) {
+          if (a.prefix)
+            a.part_ml[at] = make_float2(m, l);
+          else if (a.lse)
+            a.lse[(size_t)tok * a.heads + head] = (m + log2f(l)) * LN2;
+        }
+      }
+    } else {
+      // every CTA of the cluster is past its ring and its queries: row r goes to CTA r % nranks, behind the parts of lower ranks
+      asm volatile("bar.sync 9, 512;" ::: "memory");
+      l += s_max[0][half ^ 1][row];
+      asm volatile("barrier.cluster.wait.acquire;\nbarrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+      const int each = (ROWS + nranks - 1) / nranks;  // rows of a CTA
+      float* so = (float*)smem;
+      float2* s_ml = (float2*)(smem + ROWS * F::STRIDE * 4);
+      const int at = rank * each + row / nranks;
+      if (row < nrows) {
+        if (half == 0) {
+          const uint32_t ml_at = peer(&s_ml[at], row % nranks);
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(ml_at), "f"(has ? m : -INFINITY), "f"(has ? l : 0.f)
+                       : "memory");
+        }
+      }
+      if (has) {
+#pragma unroll
+        for (int c = 0; c < D / 64; c++) {
+          uint32_t v[32];
+          __syncwarp();
+          if constexpr (PAIR) {
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[e] = __float_as_uint(o[32 * c + e]);
+          } else {
+            tmem_ld32(obase + 32 * c, v);
+          }
+          if (row < nrows) {
+            const uint32_t to = peer(&so[at * F::STRIDE + (D / 2) * half + 32 * c], row % nranks);
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
-              *(uint4*)(a.part + at * D + 32 * c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-          } else {
-            store_row<Q>((Q*)a.out + (size_t)tok * a.out_stride + (size_t)head * D + 32 * c, v, inv);
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 4 * e), "r"(v[e]), "r"(v[e + 1]),
+                           "r"(v[e + 2]), "r"(v[e + 3])
+                           : "memory");
           }
         }
       }
-      if (live) {
-        if (a.prefix)
-          a.part_ml[at] = ml;
-        else if (a.lse)
-          a.lse[(size_t)tok * a.heads + head] = (m + log2f(l)) * LN2;
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+      // this CTA's rows, 4 columns to a thread
+      constexpr int PER = D / 4;
+      const int c = tid % PER * 4;
+      for (int k = (tid - 64) / PER; k * nranks + rank < nrows; k += 512 / PER) {
+        float M = -INFINITY, L = 0.f;
+        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int y = 0; y < nranks; y++) M = fmaxf(M, s_ml[y * each + k].x);
+        for (int y = 0; y < nranks; y++) {
+          const float2 ml = s_ml[y * each + k];
+          if (ml.x == -INFINITY) continue;  // that CTA has no part, and sent no output
+          const float wt = exp2f(ml.x - M);
+          const float4 q4 = *(const float4*)(so + (y * each + k) * F::STRIDE + c);
+          L = fmaf(wt, ml.y, L);
+          f.x = fmaf(wt, q4.x, f.x), f.y = fmaf(wt, q4.y, f.y), f.z = fmaf(wt, q4.z, f.z), f.w = fmaf(wt, q4.w, f.w);
+        }
+        const int R2 = r0 + k * nranks + rank, tok2 = R2 / a.g, head2 = kh * a.g + R2 % a.g;
+        const size_t at2 = (size_t)kh * a.rows + R2;
+        if (a.prefix) {
+          *(float4*)(a.part + at2 * D + c) = f;
+          if (c == 0) a.part_ml[at2] = make_float2(M, L);
+        } else {
+          const float inv = 1.f / L;
+          store4((Q*)a.out + (size_t)tok2 * a.out_stride + (size_t)head2 * D + c,
+                 make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv));
+          if (c == 0 && a.lse) a.lse[(size_t)tok2 * a.heads + head2] = (M + log2f(L)) * LN2;
+        }
       }
     }
     __syncwarp();
   }
-  if (nranks > 1) {
-    // the ring and the queries are no longer read: every product and every copy is done
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    float* so = (float*)smem;
-    float2* s_ml = (float2*)(smem + ROWS * F::STRIDE * 4);
-    if (warp >= 4) {
-      const int x = (warp - 4) >> 2, quarter = warp & 3, row = x * 128 + quarter * 32 + lane;
-      if (x < ntiles_x && count > 0) {
-#pragma unroll
-        for (int c = 0; c < D / 32; c++) {
-          uint32_t v[32];
-          tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + COL_O + D * x + 32 * c, v);
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *(uint4*)(so + row * F::STRIDE + 32 * c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-        }
-      }
-      s_ml[row] = ml;
-    }
+  if (nranks > 1 && warp < 2) {
+    // the issuing warps' part in the softmax warps' three cluster barriers; their copies and products are done
     __syncwarp();
-    cluster_sync();
-    if (warp >= 4) {
-      // each CTA finishes a share of the rows, 4 columns to a thread
-      constexpr int PER = D / 4;
-      const int c = tid % PER * 4;
-      for (int row = rank + (tid - 128) / PER * nranks; row < nrows; row += 256 / PER * nranks) {
-        float M = -INFINITY, L = 0.f;
-        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int y = 0; y < nranks; y++) M = fmaxf(M, ld_peer(peer(&s_ml[row].x, y)));
-        for (int y = 0; y < nranks; y++) {
-          const float mp = ld_peer(peer(&s_ml[row].x, y));
-          if (mp == -INFINITY) continue;  // that CTA has no part, and its shared memory no output
-          const float wt = exp2f(mp - M);
-          const float4 o = ld_peer4(peer(&so[row * F::STRIDE + c], y));
-          L = fmaf(wt, ld_peer(peer(&s_ml[row].y, y)), L);
-          f.x = fmaf(wt, o.x, f.x), f.y = fmaf(wt, o.y, f.y), f.z = fmaf(wt, o.z, f.z), f.w = fmaf(wt, o.w, f.w);
-        }
-        const int R = r0 + row, tok = R / a.g, head = kh * a.g + R % a.g;
-        const size_t at = (size_t)kh * a.rows + R;
-        if (a.prefix) {
-          *(float4*)(a.part + at * D + c) = f;
-          if (c == 0) a.part_ml[at] = make_float2(M, L);
-        } else {
-          const float inv = 1.f / L;
-          Q* dst = (Q*)a.out + (size_t)tok * a.out_stride + (size_t)head * D + c;
-          from_f32(f.x * inv, dst);
-          from_f32(f.y * inv, dst + 1);
-          from_f32(f.z * inv, dst + 2);
-          from_f32(f.w * inv, dst + 3);
-          if (c == 0 && a.lse) a.lse[(size_t)tok * a.heads + head] = (M + log2f(L)) * LN2;
-        }
-      }
-    }
-    __syncwarp();
-    cluster_sync();  // the peers have read this CTA's part
+    asm volatile(
+        "barrier.cluster.wait.acquire;\nbarrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n"
+        "barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -517,13 +584,7 @@ cudaError_t launch(const Rows& a, const void* k, const void* v, int ctx, int til
   auto* f = k_rows<T, D>;
   static unsigned long long done = 0;
   static std::mutex mu;
-  static bool fits = false;
-  once_per_device(done, mu, [f] {
-    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-    cudaFuncAttributes at;
-    fits = cudaFuncGetAttributes(&at, f) == cudaSuccess && at.numRegs >= REGS;  // else the split would wait for good
-  });
-  if (!fits) return cudaErrorLaunchOutOfResources;
+  once_per_device(done, mu, [f] { cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
   const int blocks = (a.rows + ROWS - 1) / ROWS;
   const int nranks = split(blocks * a.kv_heads, tiles);
   cudaLaunchConfig_t c = {};
