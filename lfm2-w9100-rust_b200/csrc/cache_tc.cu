@@ -4,17 +4,19 @@
 // prefix (the prefix half of lfm_attention_shared).
 //
 // Rows are packed: row R of a KV head is query head R % g of token (or session)
-// R / g, so every group size fills the 128-row tiles. A CTA holds two tiles of
-// rows and walks the positions in tiles of 128, with
-//   warp 0       TMA: K and V tiles into one ring of slots
-//   warp 1       TMEM and the MMAs: S_x = Q_x K^T, O_x += P_x V for tile x
-//   warps 2-9    the softmax of tile 0, warps 10-17 that of tile 1
-// While one tile is in its softmax, the products of the other run. A row is
-// shared by two threads, one for each half of its columns, which exchange
-// maxima through shared memory: with four softmax warps to a scheduler their
-// latencies overlap (one thread a row took 2.4 times as long: 311 us for 8192 bf16
-// tokens under a window of 1500). The weights P take the place of S in tensor
-// memory and enter the second product from there.
+// R / g, so every group size fills the 128-row tiles. A CTA holds one tile of
+// rows and walks the positions in tiles of 64; two CTAs share an SM, so that one
+// fills the other's waits, its start and its end. In a CTA
+//   warp 0     TMA: K and V tiles into one ring of slots
+//   warp 1     TMEM and the MMAs: S = Q K^T, O += P V
+//   warps 2-9  the softmax
+// S has two buffers: the next tile's scores are computed while this one's are in
+// the softmax. A row is shared by two threads, one for each half of its columns,
+// which exchange maxima through shared memory. The weights P take the place of S
+// in tensor memory and enter the second product from there.
+// (Two tiles of rows and 128 positions with one S each, an SM to a CTA: the chain
+// softmax - P V - Q K^T took 4400 cycles for 128 positions of bf16, 128 values,
+// of which either unit was busy for half: 282 us for 8192 tokens, window 1500.)
 //
 // 16-bit queries: O stays in tensor memory, and a row's maximum is raised, and O
 // rescaled, only when it grows by more than 2^8, which keeps every weight inside
@@ -23,8 +25,8 @@
 // instead of rounding them, a loss that grows with their number (2.2e-6 over
 // 1024 positions), so O of each tile starts from zero and is added to the
 // running output in registers.
-// Few row blocks leave SMs idle, so a cluster of CTAs may split the positions of
-// one block; each sends its part of a row to the CTA that finishes the row.
+// Few row tiles leave SMs idle, so a cluster of CTAs may split the positions of
+// one tile; each sends its part of a row to the CTA that finishes the row.
 // Every wait is bounded; one that runs out is reported and the CTA releases
 // its tensor memory.
 #include <cuda.h>
@@ -44,27 +46,27 @@ namespace {
 using namespace dev;
 using namespace tc;
 
-constexpr int THREADS = 576, KT = 128, ROWS = 256;
+constexpr int THREADS = 320, KT = 64, ROWS = 128;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float GROWTH = 8.f;  // log2 of what a row may grow before its maximum is raised
-constexpr uint32_t COLS = 512, COL_O = 256;  // S_x: [128 x, 128 x + 128); the O buffers from 256 on, D each
+constexpr uint32_t COLS = 256, COL_O = 2 * KT;  // tensor memory: two buffers of S, then those of O
 
 template <int T, int D>
 struct Cfg {
   static constexpr bool PAIR = T == T_F32;
-  static constexpr int CHUNK = 128 * 128;             // 128 rows x 64 16-bit values, swizzled
-  static constexpr int TILE = CHUNK * (D / 64);       // 128 rows x D
-  static constexpr int Q_BYTES = 2 * (PAIR ? 2 : 1) * TILE;
-  // buffers of the maxima that two threads exchange; one costs a second barrier and is taken where memory is short
-  static constexpr int MAXIMA = PAIR && D == 128 ? 1 : 2;
-  static constexpr int STATIC = MAXIMA == 1 ? 3072 : 5120;
-  static constexpr int SLOTS = std::min(6, (227 * 1024 - STATIC - Q_BYTES) / TILE);
+  static constexpr int Q_CHUNK = ROWS * 128, KV_CHUNK = KT * 128;  // rows x 64 16-bit values, swizzled
+  static constexpr int Q_TILE = Q_CHUNK * (D / 64), TILE = KV_CHUNK * (D / 64);
+  static constexpr int Q_BYTES = (PAIR ? 2 : 1) * Q_TILE;
+  static constexpr int STATIC = 3072, RESERVED = 1024;  // of the kernel's static arrays, of the system
+  // two CTAs to an SM, except for fp32 queries of 128 values, whose pairs leave no room for the second one's ring
+  static constexpr int CTAS = PAIR && D == 128 ? 1 : 2;
+  static constexpr int SLOTS = std::min(8, (228 * 1024 / CTAS - STATIC - RESERVED - Q_BYTES) / TILE);
   static constexpr int SMEM = Q_BYTES + SLOTS * TILE;
-  // O buffers of a row tile: fp32 queries fold one while the next product fills the other, where there is room
+  // O buffers: fp32 queries fold one while the next product fills the other, where there is room
   static constexpr int OBUF = PAIR && D == 64 ? 2 : 1;
   static constexpr int STRIDE = D + 4;  // floats of a row in the join: rows of one column start in different banks
-  static_assert(SLOTS >= 3 && 512 - COL_O >= 2 * OBUF * D, "memories");
-  static_assert(ROWS * (STRIDE * 4 + 8) <= Q_BYTES + SLOTS * TILE, "the join takes the place of queries and ring");
+  static_assert(SLOTS >= 4 && COL_O + OBUF * D <= COLS, "memories");
+  static_assert(ROWS * (STRIDE * 4 + 8) <= SMEM, "the join takes the place of queries and ring");
 };
 
 struct Rows {
@@ -82,23 +84,31 @@ struct Rows {
   float2* part_ml; // prefix: (m in log2 units, l)
 };
 
+// The MMAs are issued by one elected lane of a converged warp: with the branch
+// around the instruction alone, addresses and descriptors stay in uniform
+// registers (under a branch around the whole loop an MMA took ~100 cycles to
+// issue and 64 to run).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-          d),
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(db), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
+__device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -128,7 +138,7 @@ __device__ __forceinline__ void st_piece(uint8_t* chunk, int r, int piece, uint4
 
 // The position tiles of a block of rows: the sinks in front of the window, then
 // the positions from the first row's window to the last row. A tile has `width`
-// columns (a multiple of 32) of which the first `valid` exist.
+// columns (32 or 64) of which the first `valid` exist.
 struct Tiles {
   int hi, lo, end, ns, n;
   __device__ __forceinline__ Tiles(int hi_, int lo_, int end_) : hi(hi_), lo(lo_), end(end_) {
@@ -141,7 +151,7 @@ struct Tiles {
 };
 
 template <int T, int D>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     k_rows(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Rows a) {
   using F = Cfg<T, D>;
   using Q = typename Types<T>::Q;
@@ -150,21 +160,21 @@ __global__ void __launch_bounds__(THREADS, 1)
   constexpr uint32_t BF = std::is_same<C, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* slots = smem + F::Q_BYTES;
-  __shared__ uint64_t q_full, full[F::SLOTS], empty[F::SLOTS], s_full[2], p_full[2];
+  __shared__ uint64_t q_full, full[F::SLOTS], empty[F::SLOTS], s_full[2], p_full[2], o_full[2];
   __shared__ uint32_t tmem_at;
-  __shared__ float s_max[F::MAXIMA][2][ROWS];  // [tile parity][half][row]
+  __shared__ float s_max[2][2][ROWS];  // [tile parity][half][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
   const int r0 = (int)(gridDim.z - 1 - blockIdx.z) * ROWS;  // the longest rows first
   const int nrows = min(ROWS, a.rows - r0);
-  const int ntiles_x = nrows > 128 ? 2 : 1;
   const int p0 = a.prefix ? 0 : a.start + r0 / a.g, p1 = a.prefix ? 0 : a.start + (r0 + nrows - 1) / a.g;
   const int lo0 = a.prefix ? 0 : window_first(p0, a.window);
   const Tiles tiles(a.prefix ? 0 : min(a.sinks, lo0), lo0, a.prefix ? a.len : p1 + 1);
   const int i0 = (int)((long long)tiles.n * rank / nranks), i1 = (int)((long long)tiles.n * (rank + 1) / nranks);
+  const int count = i1 - i0;
 
   if (tid == 0) {
-    mbar_init(&q_full, 16);
+    mbar_init(&q_full, 8);
     for (int i = 0; i < F::SLOTS; i++) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -172,6 +182,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int x = 0; x < 2; x++) {
       mbar_init(&s_full[x], 1);
       mbar_init(&p_full[x], 8);
+      mbar_init(&o_full[x], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -180,7 +191,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
-  const int count = i1 - i0;
   if (nranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   if (warp < 2) {
@@ -194,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         mbar_expect_tx(&full[st], F::TILE);
 #pragma unroll
         for (int c = 0; c < D / 64; c++)
-          tma_load_3d(slots + st * F::TILE + c * F::CHUNK, map, 64 * c, j, kh, &full[st]);
+          tma_load_3d(slots + st * F::TILE + c * F::KV_CHUNK, map, 64 * c, j, kh, &full[st]);
         n++;
       };
       for (int i = i0; i < i1 && ok; i++) {
@@ -206,84 +216,73 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = max(0, n - F::SLOTS); i < n; i++) mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr);
     } else if (warp == 1 && count > 0) {
       // -------------------------------------------------------------- MMAs
-      constexpr uint32_t IDESC_PV = idesc_f16(128, D, true) | BF;
-      bool ok = mbar_wait(&q_full, 0, nullptr);
-      const bool one = lane == 0;
-      auto qk = [&](int x, int i) {  // tile i of the block, slot 2 (i - i0)
-        const int n = 2 * (i - i0), st = n % F::SLOTS;
-        if (!ok || !(ok = mbar_wait(&full[st], (n / F::SLOTS) & 1, nullptr))) return;
-        tc_fence_after();
-        if (one) {
-          const uint32_t idesc = idesc_f16(128, tiles.width(i), false) | BF;
-          const uint32_t d = tmem + 128 * x, kb = smem_u32(slots + st * F::TILE);
-          const uint32_t qb = smem_u32(smem) + x * (F::Q_BYTES / 2);
-#pragma unroll
-          for (int h = 0; h < (PAIR ? 2 : 1); h++)
-#pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) {
-              const uint32_t off = (kk >> 2) * F::CHUNK + (kk & 3) * 32;
-              mma_f16(d, smem_desc_sw128(qb + (PAIR ? 1 - h : 0) * F::TILE + off), smem_desc_sw128(kb + off), idesc,
-                      h || kk);
-            }
-        }
+      constexpr uint32_t IDESC_PV = idesc_f16(ROWS, D, true) | BF;
+      const uint32_t tm = uniform(tmem), q0 = uniform(smem_u32(smem)), ring = uniform(smem_u32(slots));
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, nullptr));
       };
-      auto pv = [&](int x, int i) {
-        const int n = 2 * (i - i0) + 1, st = n % F::SLOTS;
-        if (!ok || !(ok = mbar_wait(&full[st], (n / F::SLOTS) & 1, nullptr))) return;
-        uint8_t* vb = slots + st * F::TILE;
-        const int width = tiles.width(i), valid = tiles.valid(i);
-        if (x == 0 && valid < width) {  // rows that no query sees: their weights are 0, so they must be finite
+      bool ok = wait(&q_full, 0);
+      auto qk = [&](int k) {  // this CTA's k-th tile: K in the 2 k-th slot
+        const int st = 2 * k % F::SLOTS;
+        if (!ok || !(ok = wait(&full[st], (2 * k / F::SLOTS) & 1))) return;
+        tc_fence_after();
+        const uint32_t idesc = idesc_f16(ROWS, tiles.width(i0 + k), false) | BF;
+        const uint32_t d = tm + KT * (k & 1);
+        const uint64_t kb = smem_desc_sw128(ring + st * F::TILE), qb = smem_desc_sw128(q0);
+#pragma unroll
+        for (int h = 0; h < (PAIR ? 2 : 1); h++)
+#pragma unroll
+          for (int kk = 0; kk < D / 16; kk++)
+            mma_ss(d, qb + (((PAIR ? 1 - h : 0) * F::Q_TILE + (kk >> 2) * F::Q_CHUNK + (kk & 3) * 32) >> 4),
+                   kb + (((kk >> 2) * F::KV_CHUNK + (kk & 3) * 32) >> 4), idesc, h || kk);
+        commit(&s_full[k & 1]);
+        commit(&empty[st]);
+      };
+      auto pv = [&](int k) {  // V in the slot behind K's
+        const int st = (2 * k + 1) % F::SLOTS;
+        if (!ok || !(ok = wait(&full[st], ((2 * k + 1) / F::SLOTS) & 1))) return;
+        const int width = tiles.width(i0 + k), valid = tiles.valid(i0 + k);
+        if (valid < width) {  // rows that no query sees: their weights are 0, so they must be finite
+          uint8_t* vb = slots + st * F::TILE;
 #pragma unroll
           for (int c = 0; c < D / 64; c++)
             for (int o = valid * 128 + 16 * lane; o < width * 128; o += 512)
-              *(uint4*)(vb + c * F::CHUNK + o) = make_uint4(0, 0, 0, 0);
+              *(uint4*)(vb + c * F::KV_CHUNK + o) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
           __syncwarp();
         }
+        if (!(ok = wait(&p_full[k & 1], (k >> 1) & 1))) return;
         tc_fence_after();
-        if (one) {
-          const uint32_t d = tmem + COL_O + D * (F::OBUF * x + ((i - i0) & (F::OBUF - 1)));
-          const uint32_t p = tmem + 128 * x, v = smem_u32(vb);
-          for (int h = 0; h < (PAIR ? 2 : 1); h++)  // 32 columns of S hold 16 columns of weights, and behind them their low parts
-            for (int kk = 0; kk < width / 16; kk++)
-              mma_ts(d, p + 32 * (kk >> 1) + 8 * (kk & 1) + (PAIR && h == 0 ? 16 : 0),
-                     smem_desc_mn_sw128(v + kk * 2048, F::CHUNK), IDESC_PV, (!PAIR && i > i0) || h || kk);
-        }
+        const uint32_t d = tm + COL_O + D * (k & (F::OBUF - 1)), p = tm + KT * (k & 1);
+        const uint64_t v = smem_desc_mn_sw128(ring + st * F::TILE, F::KV_CHUNK);
+#pragma unroll
+        for (int h = 0; h < (PAIR ? 2 : 1); h++)  // 32 columns of S hold 16 columns of weights, and behind them their low parts
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; kk++)
+            if (kk < 2 || 16 * kk < width)
+              mma_ts(d, p + 32 * (kk >> 1) + 8 * (kk & 1) + (PAIR && h == 0 ? 16 : 0), v + kk * (2048 >> 4), IDESC_PV,
+                     h || kk ? 1u : (!PAIR && k > 0));
+        commit(&o_full[k & 1]);
+        commit(&empty[st]);
       };
-      for (int x = 0; x < ntiles_x; x++) {
-        qk(x, i0);
-        if (one && ok) mma_commit(&s_full[x]);
+      qk(0);
+      for (int k = 0; k < count && ok; k++) {
+        if (k + 1 < count) qk(k + 1);  // into the buffer whose weights the last product has taken: MMAs run in order
+        pv(k);
       }
-      if (one && ok) mma_commit(&empty[0]);
-      for (int i = i0; i < i1 && ok; i++) {
-        for (int x = 0; x < ntiles_x && ok; x++) {
-          if (!(ok = mbar_wait(&p_full[x], (i - i0) & 1, nullptr))) break;
-          tc_fence_after();
-          pv(x, i);
-          if (i + 1 < i1) qk(x, i + 1);
-          if (one && ok) mma_commit(&s_full[x]);  // S of the next tile, and O of this one
-        }
-        if (one && ok) {
-          mma_commit(&empty[(2 * (i - i0) + 1) % F::SLOTS]);
-          if (i + 1 < i1) mma_commit(&empty[(2 * (i - i0) + 2) % F::SLOTS]);
-        }
-        __syncwarp();
-      }
-      if (!ok && one) report(BAD_WAIT);
+      if (!ok && lane == 0) report(BAD_WAIT);
     }
   } else {
     // -------------------------------------------------------------- softmax
-    const int x = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1, quarter = warp & 3;  // TMEM lanes by warp % 4
-    const int rt = quarter * 32 + lane, row = x * 128 + rt;
+    const int half = ((warp - 2) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;  // TMEM lanes by warp % 4
     const int R = r0 + min(row, nrows - 1), tok = R / a.g, head = kh * a.g + R % a.g;
     const bool live = row < nrows;
     {
       const Q* q = (const Q*)a.q + (size_t)tok * a.q_stride + (size_t)head * D;
-      uint8_t* dst = smem + x * (F::Q_BYTES / 2);
 #pragma unroll
       for (int i = 0; i < D / 16; i++) {
         const int c = half * (D / 16) + i;
-        uint8_t* chunk = dst + (c >> 3) * F::CHUNK;
+        uint8_t* chunk = smem + (c >> 3) * F::Q_CHUNK;
         if constexpr (PAIR) {
           const float4 u = *(const float4*)(q + 8 * c), v = *(const float4*)(q + 8 * c + 4);
           const float f[8] = {u.x * a.scale2, u.y * a.scale2, u.z * a.scale2, u.w * a.scale2,
@@ -294,10 +293,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             h[e] = pack(__half(), f[2 * e], f[2 * e + 1]);
             l[e] = rest(h[e], f[2 * e], f[2 * e + 1]);
           }
-          st_piece(chunk, rt, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
-          st_piece(chunk + F::TILE, rt, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
+          st_piece(chunk, row, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
+          st_piece(chunk + F::Q_TILE, row, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
         } else {
-          st_piece(chunk, rt, c & 7, *(const uint4*)(q + 8 * c));
+          st_piece(chunk, row, c & 7, *(const uint4*)(q + 8 * c));
         }
       }
       fence_async_smem();
@@ -305,124 +304,128 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (lane == 0) mbar_arrive(&q_full);
     }
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t sbase = mine + 128 * x + 64 * half, obase = mine + COL_O + D * F::OBUF * x + (D / 2) * half;
+    const uint32_t obase = mine + COL_O + (D / 2) * half;
     const float sc = PAIR ? 1.f : a.scale2;
     const int p = a.start + tok;
     const int wlo = a.window > 0 ? p - a.window + 1 : -0x40000000;
-    const int pair = 1 + 4 * x + quarter;  // the named barrier of the two warps that share these rows
+    const int pair = 1 + quarter;  // the named barrier of the two warps that share these rows
     float m = -INFINITY, l = 0.f, alpha_last = 0.f;
     float o[PAIR ? D / 2 : 1] = {};  // fp32 queries: this half's columns of the running output
     bool ok = true;
-    auto fold = [&](int n) {  // O of the n-th tile, whose maximum came with alpha_last
+    // The k-th product has been added. Two barriers in turn: a warp that folds after it has handed on its weights may
+    // come here when the next product is done too, and one barrier's parity would have come round.
+    auto wait_o = [&](int k) {
+      if (ok) ok = mbar_wait(&o_full[k & 1], (k >> 1) & 1, nullptr);
+      tc_fence_after();
+    };
+    auto fold = [&](int k) {  // O of the k-th tile, whose maximum came with alpha_last
       if constexpr (PAIR) {
+        wait_o(k);
+        __syncwarp();
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
           uint32_t v[16];
-          tmem_ld16_nowait(obase + D * (n & (F::OBUF - 1)) + 16 * c, v);
+          tmem_ld16_nowait(obase + D * (k & (F::OBUF - 1)) + 16 * c, v);
           tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 16; e++) o[16 * c + e] = fmaf(o[16 * c + e], alpha_last, __uint_as_float(v[e]));
         }
       }
     };
-    if (x < ntiles_x) {
-      for (int i = i0; i < i1; i++) {
-        const int n = i - i0;
-        if (ok) ok = mbar_wait(&s_full[x], n & 1, nullptr);  // a warp that gave up still meets its partner below
-        tc_fence_after();
-        const int j0 = tiles.first(i) + 64 * half, width = tiles.width(i) - 64 * half, valid = tiles.valid(i) - 64 * half;
-        // the columns that some row of the block does not see
+    for (int k = 0; k < count; k++) {
+      const int i = i0 + k;
+      if (ok) ok = mbar_wait(&s_full[k & 1], (k >> 1) & 1, nullptr);  // a warp that gave up still meets its partner below
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t sbase = mine + KT * (k & 1) + 32 * half;
+      const int j0 = tiles.first(i) + 32 * half, valid = tiles.valid(i) - 32 * half;
+      const bool some = valid > 0;
+      uint32_t v[32];
+      float mx = -INFINITY;
+      if (some) {
+        tmem_ld32(sbase, v);
+        // the columns that some row of the tile does not see
         const bool full_tile =
-            valid >= 64 && (a.prefix || i < tiles.ns ||
-                            (j0 + 63 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + 64 <= a.sinks)));
-        int cmax = valid - 1, cmin = -1, csink = 0;
-        if (!a.prefix && i >= tiles.ns) cmax = min(cmax, p - j0), cmin = wlo - j0, csink = a.sinks - j0;
-        // S is read twice, for the maximum and for the weights: a thread's 64 columns do not fit beside the rest of
-        // its registers (292 bytes of spills for 16-bit queries)
-        auto take = [&](int c, uint32_t(&v)[32]) {
-          tmem_ld32(sbase + 32 * c, v);
-          if (!full_tile) {
+            valid >= 32 && (a.prefix || i < tiles.ns ||
+                            (j0 + 31 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + 32 <= a.sinks)));
+        if (!full_tile) {
+          int cmax = valid - 1, cmin = -1, csink = 0;
+          if (!a.prefix && i >= tiles.ns) cmax = min(cmax, p - j0), cmin = wlo - j0, csink = a.sinks - j0;
 #pragma unroll
-            for (int e = 0; e < 32; e++)
-              if (!(32 * c + e <= cmax && (32 * c + e >= cmin || 32 * c + e < csink))) v[e] = 0xff800000u;
-          }
-        };
-        float mx = -INFINITY, my = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-          if (32 * c < width) {
-            uint32_t v[32];
-            take(c, v);
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-              my = max3(my, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
-            }
-          }
-        mx = fmaxf(mx, my);
-        float(&exchange)[2][ROWS] = s_max[n & (F::MAXIMA - 1)];
-        exchange[half][row] = mx;
-        asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-        mx = fmaxf(mx, exchange[half ^ 1][row]) * sc;
-        if (F::MAXIMA == 1) asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-        float alpha = 1.f;
-        if (PAIR || __any_sync(0xffffffffu, mx > m + GROWTH)) {
-          const float mn = fmaxf(m, mx);
-          alpha = m == -INFINITY ? 0.f : exp2_fast(m - mn);
-          if (!PAIR && n > 0) {
-#pragma unroll
-            for (int c = 0; c < D / 64; c++) {
-              uint32_t v[32];
-              tmem_ld32(obase + 32 * c, v);
-#pragma unroll
-              for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-              tmem_st32(obase + 32 * c, v);
-            }
-          }
-          l *= alpha;
-          m = mn;
+          for (int e = 0; e < 32; e++)
+            if (!(e <= cmax && (e >= cmin || e < csink))) v[e] = 0xff800000u;
         }
-        if (F::OBUF == 1 && n > 0) fold(n - 1);
+        float my = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          my = max3(my, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+        }
+        mx = fmaxf(mx, my);
+      }
+      float(&exchange)[2][ROWS] = s_max[k & 1];
+      exchange[half][row] = mx;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
+      mx = fmaxf(mx, exchange[half ^ 1][row]) * sc;
+      float alpha = 1.f;
+      if (PAIR || __any_sync(0xffffffffu, mx > m + GROWTH)) {
+        const float mn = fmaxf(m, mx);
+        alpha = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+        if (!PAIR && k > 0) {
+          wait_o(k - 1);
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < D / 32; c++) {
+            uint32_t w[16];
+            tmem_ld16_nowait(obase + 16 * c, w);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
+            tmem_st16(obase + 16 * c, w);
+          }
+        }
+        l *= alpha;
+        m = mn;
+      }
+      if (F::OBUF == 1 && k > 0) fold(k - 1);
+      if (some) {
         const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: its weights are all 0
         const uint64_t sc2 = two(sc, sc), ms2 = two(-ms, -ms);
         uint64_t la = 0, lb = 0;  // pairs of 0.f
+        uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int c = 0; c < 2; c++)
-          if (32 * c < width) {
-            uint32_t v[32], hi[16], lo[16];
-            take(c, v);
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-              const float2 z = one(fma2(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, ms2));
-              const float u = exp2_fast(z.x), w = exp2_fast(z.y);
-              if (e & 1)
-                lb = add2(lb, two(u, w));
-              else
-                la = add2(la, two(u, w));
-              hi[e] = pack(C(), u, w);
-              if constexpr (PAIR) lo[e] = rest(hi[e], u, w);
-            }
-            tmem_st16(sbase + 32 * c, hi);
-            if constexpr (PAIR) tmem_st16(sbase + 32 * c + 16, lo);
-          }
+        for (int e = 0; e < 16; e++) {
+          const float2 z = one(fma2(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, ms2));
+          const float u = exp2_fast(z.x), w = exp2_fast(z.y);
+          if (e & 1)
+            lb = add2(lb, two(u, w));
+          else
+            la = add2(la, two(u, w));
+          hi[e] = pack(C(), u, w);
+          if constexpr (PAIR) lo[e] = rest(hi[e], u, w);
+        }
+        tmem_st16(sbase, hi);
+        if constexpr (PAIR) tmem_st16(sbase + 16, lo);
         const float2 sum = one(add2(la, lb));
         l += sum.x + sum.y;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
-        if (F::OBUF == 2 && n > 0) fold(n - 1);
-        alpha_last = alpha;
       }
-      if (count > 0) {
-        if (ok) ok = mbar_wait(&s_full[x], count & 1, nullptr);  // the last product
-        tc_fence_after();
-        if (PAIR) fold(count - 1);
-      }
-      if (!ok && lane == 0) report(BAD_WAIT);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[k & 1]);
+      if (F::OBUF == 2 && k > 0) fold(k - 1);
+      alpha_last = alpha;
     }
+    const bool has = count > 0;
+    if (has) {
+      if constexpr (PAIR)
+        fold(count - 1);
+      else
+        wait_o(count - 1);
+    }
+    if (!ok && lane == 0) report(BAD_WAIT);
     // ------------------------------------------------------------ epilogue
-    const bool has = x < ntiles_x && count > 0;
+    // the partner has read the last tile's maxima: the product it took part in is done
     s_max[0][half][row] = l;
     if (nranks == 1) {
       asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     } else {
       // every CTA of the cluster is past its ring and its queries: row r goes to CTA r % nranks, behind the parts of lower ranks
-      asm volatile("bar.sync 9, 512;" ::: "memory");
+      asm volatile("bar.sync 9, 256;" ::: "memory");
       l += s_max[0][half ^ 1][row];
       asm volatile("barrier.cluster.wait.acquire;\nbarrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
       const int each = (ROWS + nranks - 1) / nranks;  // rows of a CTA
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // this CTA's rows, 4 columns to a thread
       constexpr int PER = D / 4;
       const int c = tid % PER * 4;
-      for (int k = (tid - 64) / PER; k * nranks + rank < nrows; k += 512 / PER) {
+      for (int k = (tid - 64) / PER; k * nranks + rank < nrows; k += 256 / PER) {
         float M = -INFINITY, L = 0.f;
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int y = 0; y < nranks; y++) M = fmaxf(M, s_ml[y * each + k].x);
@@ -554,7 +557,7 @@ EncodeFn encode_fn() {
   return fn;
 }
 
-// A cache slot [kv head][position][d] of 16-bit values, read in boxes of 64 values x 128 positions of one head.
+// A cache slot [kv head][position][d] of 16-bit values, read in boxes of 64 values x 64 positions of one head.
 cudaError_t map_cache(CUtensorMap* map, const void* base, int kv_heads, int ctx, int d) {
   EncodeFn fn = encode_fn();
   if (!fn) return cudaErrorNotSupported;
@@ -570,7 +573,7 @@ cudaError_t map_cache(CUtensorMap* map, const void* base, int kv_heads, int ctx,
 // CTAs that split one block's positions: as many as fill the SMs, each with a tile of its own at least.
 int split(int blocks, int tiles) {
   int n = 1;
-  while (n < 8 && 2 * n * blocks <= 148 && 2 * n <= tiles) n *= 2;
+  while (n < 8 && 2 * n * blocks <= 2 * 148 && 2 * n <= tiles) n *= 2;
   return n;
 }
 
