@@ -7,7 +7,7 @@
 // R / g, so every group size fills the 128-row tiles. A CTA holds one tile of
 // rows and walks the positions in tiles of 64; two CTAs share an SM, so that one
 // fills the other's waits, its start and its end. In a CTA
-//   warp 0     TMA: K and V tiles into one ring of slots
+//   warp 0     TMA: K and V tiles into a ring each
 //   warp 1     TMEM and the MMAs: S = Q K^T, O += P V
 //   warps 2-9  the softmax
 // S has two buffers: the next tile's scores are computed while this one's are in
@@ -60,12 +60,12 @@ struct Cfg {
   static constexpr int STATIC = 3072, RESERVED = 1024;  // of the kernel's static arrays, of the system
   // two CTAs to an SM, except for fp32 queries of 128 values, whose pairs leave no room for the second one's ring
   static constexpr int CTAS = PAIR && D == 128 ? 1 : 2;
-  static constexpr int SLOTS = std::min(8, (228 * 1024 / CTAS - STATIC - RESERVED - Q_BYTES) / TILE);
-  static constexpr int SMEM = Q_BYTES + SLOTS * TILE;
+  static constexpr int RING = std::min(4, (228 * 1024 / CTAS - STATIC - RESERVED - Q_BYTES) / (2 * TILE));  // K and V tiles each
+  static constexpr int SMEM = Q_BYTES + 2 * RING * TILE;
   // O buffers: fp32 queries fold one while the next product fills the other, where there is room
   static constexpr int OBUF = PAIR && D == 64 ? 2 : 1;
   static constexpr int STRIDE = D + 4;  // floats of a row in the join: rows of one column start in different banks
-  static_assert(SLOTS >= 4 && COL_O + OBUF * D <= COLS, "memories");
+  static_assert(RING >= 2 && COL_O + OBUF * D <= COLS, "memories");
   static_assert(ROWS * (STRIDE * 4 + 8) <= SMEM, "the join takes the place of queries and ring");
 };
 
@@ -136,18 +136,34 @@ __device__ __forceinline__ void st_piece(uint8_t* chunk, int r, int piece, uint4
   *(uint4*)(chunk + r * 128 + ((piece ^ (r & 7)) << 4)) = v;
 }
 
+// The n lowest bits.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+}
+
 // The position tiles of a block of rows: the sinks in front of the window, then
 // the positions from the first row's window to the last row. A tile has `width`
-// columns (32 or 64) of which the first `valid` exist.
+// columns (32 or 64) of which the first `valid` exist. Every row sees all of the
+// tiles [all0, all1).
 struct Tiles {
-  int hi, lo, end, ns, n;
-  __device__ __forceinline__ Tiles(int hi_, int lo_, int end_) : hi(hi_), lo(lo_), end(end_) {
+  int hi, lo, end, ns, n, all0, all1;
+  __device__ __forceinline__ Tiles(const Rows& a, int r0, int nrows) {
+    int p0 = 0, p1 = 0;
+    lo = hi = 0, end = a.len;
+    if (!a.prefix) {
+      p0 = a.start + r0 / a.g, p1 = a.start + (r0 + nrows - 1) / a.g;
+      lo = window_first(p0, a.window), hi = min(a.sinks, lo), end = p1 + 1;
+    }
     ns = (hi + KT - 1) / KT;
     n = ns + (end - lo + KT - 1) / KT;
+    // behind the start of the last row's window, and not past the first row
+    all0 = ns + (a.window > 0 ? (max(window_first(p1, a.window) - lo, 0) + KT - 1) / KT : 0);
+    all1 = ns + ((a.prefix ? end : p0 + 1) - lo) / KT;
   }
+  __device__ __forceinline__ bool all(int i) const { return i >= all0 && i < all1; }
   __device__ __forceinline__ int first(int i) const { return i < ns ? i * KT : lo + (i - ns) * KT; }
   __device__ __forceinline__ int valid(int i) const { return min(KT, (i < ns ? hi : end) - first(i)); }
-  __device__ __forceinline__ int width(int i) const { return (valid(i) + 31) & ~31; }
+  __device__ __forceinline__ int width(int i) const { return all(i) || valid(i) > 32 ? 64 : 32; }
 };
 
 template <int T, int D>
@@ -159,31 +175,30 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   constexpr bool PAIR = F::PAIR;
   constexpr uint32_t BF = std::is_same<C, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* slots = smem + F::Q_BYTES;
-  __shared__ uint64_t q_full, full[F::SLOTS], empty[F::SLOTS], s_full[2], p_full[2], o_full[2];
+  uint8_t* ring = smem + F::Q_BYTES;  // K and V of ring place 0, of place 1, ...
+  // s_full: scores computed, and with them the K tile free again; o_full: output added, and with it the V tile. One of
+  // each for every ring place, because a parity must not come round before its last reader has come by: a softmax warp
+  // may wait for a product when the next one is done too.
+  __shared__ uint64_t q_full, k_full[F::RING], v_full[F::RING], s_full[F::RING], o_full[F::RING], p_full[2];
   __shared__ uint32_t tmem_at;
   __shared__ float s_max[2][2][ROWS];  // [tile parity][half][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
   const int r0 = (int)(gridDim.z - 1 - blockIdx.z) * ROWS;  // the longest rows first
   const int nrows = min(ROWS, a.rows - r0);
-  const int p0 = a.prefix ? 0 : a.start + r0 / a.g, p1 = a.prefix ? 0 : a.start + (r0 + nrows - 1) / a.g;
-  const int lo0 = a.prefix ? 0 : window_first(p0, a.window);
-  const Tiles tiles(a.prefix ? 0 : min(a.sinks, lo0), lo0, a.prefix ? a.len : p1 + 1);
+  const Tiles tiles(a, r0, nrows);
   const int i0 = (int)((long long)tiles.n * rank / nranks), i1 = (int)((long long)tiles.n * (rank + 1) / nranks);
   const int count = i1 - i0;
 
   if (tid == 0) {
     mbar_init(&q_full, 8);
-    for (int i = 0; i < F::SLOTS; i++) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
+    for (int i = 0; i < F::RING; i++) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&o_full[i], 1);
     }
-    for (int x = 0; x < 2; x++) {
-      mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 8);
-      mbar_init(&o_full[x], 1);
-    }
+    for (int i = 0; i < 2; i++) mbar_init(&p_full[i], 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&tmem_at, COLS);
@@ -196,65 +211,69 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   if (warp < 2) {
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
-      int n = 0;
       bool ok = true;
-      auto load = [&](const CUtensorMap* map, int j) {
-        const int st = n % F::SLOTS;
-        if (n >= F::SLOTS && !(ok = mbar_wait(&empty[st], (n / F::SLOTS - 1) & 1, nullptr))) return;
+      int nk = 0, nv = 0;
+      auto load = [&](const CUtensorMap* map, int& k, uint64_t* full, uint64_t* free, int at) {
+        const int st = k % F::RING;
+        if (!ok || (k >= F::RING && !(ok = mbar_wait(&free[st], (k / F::RING - 1) & 1, nullptr)))) return;
         mbar_expect_tx(&full[st], F::TILE);
 #pragma unroll
         for (int c = 0; c < D / 64; c++)
-          tma_load_3d(slots + st * F::TILE + c * F::KV_CHUNK, map, 64 * c, j, kh, &full[st]);
-        n++;
+          tma_load_3d(ring + 2 * st * F::TILE + at + c * F::KV_CHUNK, map, 64 * c, tiles.first(i0 + k), kh, &full[st]);
+        k++;
       };
-      for (int i = i0; i < i1 && ok; i++) {
-        load(&map_k, tiles.first(i));
-        if (ok) load(&map_v, tiles.first(i));
+      // in the order in which the places come free: the scores of tile k + 1 are computed before the output of tile k - 1
+      while (ok && nv < count) {
+        if (nk < count) load(&map_k, nk, k_full, s_full, 0);
+        if (nk > nv + 1 || nk == count) load(&map_v, nv, v_full, o_full, F::TILE);
       }
       if (!ok) report(BAD_WAIT);
       // the copies land before the CTA's shared memory is used for anything else
-      for (int i = max(0, n - F::SLOTS); i < n; i++) mbar_wait(&full[i % F::SLOTS], (i / F::SLOTS) & 1, nullptr);
+      for (int k = max(0, nk - F::RING); k < nk; k++) mbar_wait(&k_full[k % F::RING], (k / F::RING) & 1, nullptr);
+      for (int k = max(0, nv - F::RING); k < nv; k++) mbar_wait(&v_full[k % F::RING], (k / F::RING) & 1, nullptr);
     } else if (warp == 1 && count > 0) {
       // -------------------------------------------------------------- MMAs
       constexpr uint32_t IDESC_PV = idesc_f16(ROWS, D, true) | BF;
-      const uint32_t tm = uniform(tmem), q0 = uniform(smem_u32(smem)), ring = uniform(smem_u32(slots));
+      const uint32_t tm = uniform(tmem), q0 = uniform(smem_u32(smem)), ring0 = uniform(smem_u32(ring));
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, nullptr));
       };
       bool ok = wait(&q_full, 0);
-      auto qk = [&](int k) {  // this CTA's k-th tile: K in the 2 k-th slot
-        const int st = 2 * k % F::SLOTS;
-        if (!ok || !(ok = wait(&full[st], (2 * k / F::SLOTS) & 1))) return;
+      auto qk = [&](int k) {  // this CTA's k-th tile
+        const int st = k % F::RING;
+        if (k >= count || !ok || !(ok = wait(&k_full[st], (k / F::RING) & 1))) return;
         tc_fence_after();
         const uint32_t idesc = idesc_f16(ROWS, tiles.width(i0 + k), false) | BF;
         const uint32_t d = tm + KT * (k & 1);
-        const uint64_t kb = smem_desc_sw128(ring + st * F::TILE), qb = smem_desc_sw128(q0);
+        const uint64_t kb = smem_desc_sw128(ring0 + 2 * st * F::TILE), qb = smem_desc_sw128(q0);
 #pragma unroll
         for (int h = 0; h < (PAIR ? 2 : 1); h++)
 #pragma unroll
           for (int kk = 0; kk < D / 16; kk++)
             mma_ss(d, qb + (((PAIR ? 1 - h : 0) * F::Q_TILE + (kk >> 2) * F::Q_CHUNK + (kk & 3) * 32) >> 4),
                    kb + (((kk >> 2) * F::KV_CHUNK + (kk & 3) * 32) >> 4), idesc, h || kk);
-        commit(&s_full[k & 1]);
-        commit(&empty[st]);
+        commit(&s_full[st]);
       };
-      auto pv = [&](int k) {  // V in the slot behind K's
-        const int st = (2 * k + 1) % F::SLOTS;
-        if (!ok || !(ok = wait(&full[st], ((2 * k + 1) / F::SLOTS) & 1))) return;
-        const int width = tiles.width(i0 + k), valid = tiles.valid(i0 + k);
+      qk(0);
+      qk(1);
+      for (int k = 0; k < count && ok; k++) {
+        const int st = k % F::RING;
+        if (!(ok = wait(&v_full[st], (k / F::RING) & 1))) break;
+        const uint32_t vb = ring0 + (2 * st + 1) * F::TILE;
+        const int width = tiles.width(i0 + k), valid = tiles.all(i0 + k) ? KT : tiles.valid(i0 + k);
         if (valid < width) {  // rows that no query sees: their weights are 0, so they must be finite
-          uint8_t* vb = slots + st * F::TILE;
+          uint8_t* v = ring + (2 * st + 1) * F::TILE;
 #pragma unroll
           for (int c = 0; c < D / 64; c++)
             for (int o = valid * 128 + 16 * lane; o < width * 128; o += 512)
-              *(uint4*)(vb + c * F::KV_CHUNK + o) = make_uint4(0, 0, 0, 0);
+              *(uint4*)(v + c * F::KV_CHUNK + o) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
           __syncwarp();
         }
-        if (!(ok = wait(&p_full[k & 1], (k >> 1) & 1))) return;
+        if (!(ok = wait(&p_full[k & 1], (k >> 1) & 1))) break;
         tc_fence_after();
         const uint32_t d = tm + COL_O + D * (k & (F::OBUF - 1)), p = tm + KT * (k & 1);
-        const uint64_t v = smem_desc_mn_sw128(ring + st * F::TILE, F::KV_CHUNK);
+        const uint64_t v = smem_desc_mn_sw128(vb, F::KV_CHUNK);
 #pragma unroll
         for (int h = 0; h < (PAIR ? 2 : 1); h++)  // 32 columns of S hold 16 columns of weights, and behind them their low parts
 #pragma unroll
@@ -262,13 +281,11 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
             if (kk < 2 || 16 * kk < width)
               mma_ts(d, p + 32 * (kk >> 1) + 8 * (kk & 1) + (PAIR && h == 0 ? 16 : 0), v + kk * (2048 >> 4), IDESC_PV,
                      h || kk ? 1u : (!PAIR && k > 0));
-        commit(&o_full[k & 1]);
-        commit(&empty[st]);
-      };
-      qk(0);
-      for (int k = 0; k < count && ok; k++) {
-        if (k + 1 < count) qk(k + 1);  // into the buffer whose weights the last product has taken: MMAs run in order
-        pv(k);
+        // The scores of the tile after next take the place of these weights: MMAs run in order. Its commit goes first
+        // where O is rarely waited for (a commit costs the issuing warp ~200 cycles).
+        if (PAIR) commit(&o_full[st]);
+        qk(k + 2);
+        if (!PAIR) commit(&o_full[st]);
       }
       if (!ok && lane == 0) report(BAD_WAIT);
     }
@@ -312,10 +329,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     float m = -INFINITY, l = 0.f, alpha_last = 0.f;
     float o[PAIR ? D / 2 : 1] = {};  // fp32 queries: this half's columns of the running output
     bool ok = true;
-    // The k-th product has been added. Two barriers in turn: a warp that folds after it has handed on its weights may
-    // come here when the next product is done too, and one barrier's parity would have come round.
-    auto wait_o = [&](int k) {
-      if (ok) ok = mbar_wait(&o_full[k & 1], (k >> 1) & 1, nullptr);
+    auto wait_o = [&](int k) {  // the k-th product has been added
+      if (ok) ok = mbar_wait(&o_full[k % F::RING], (k / F::RING) & 1, nullptr);
       tc_fence_after();
     };
     auto fold = [&](int k) {  // O of the k-th tile, whose maximum came with alpha_last
@@ -334,34 +349,40 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     };
     for (int k = 0; k < count; k++) {
       const int i = i0 + k;
-      if (ok) ok = mbar_wait(&s_full[k & 1], (k >> 1) & 1, nullptr);  // a warp that gave up still meets its partner below
+      if (ok) ok = mbar_wait(&s_full[k % F::RING], (k / F::RING) & 1, nullptr);  // a warp that gave up still meets its partner below
       __syncwarp();
       tc_fence_after();
       const uint32_t sbase = mine + KT * (k & 1) + 32 * half;
-      const int j0 = tiles.first(i) + 32 * half, valid = tiles.valid(i) - 32 * half;
-      const bool some = valid > 0;
+      bool some = true;  // this half has columns
       uint32_t v[32];
       float mx = -INFINITY;
-      if (some) {
-        tmem_ld32(sbase, v);
-        // the columns that some row of the tile does not see
-        const bool full_tile =
-            valid >= 32 && (a.prefix || i < tiles.ns ||
-                            (j0 + 31 <= p0 && (a.window == 0 || j0 > p1 - a.window || j0 + 32 <= a.sinks)));
-        if (!full_tile) {
-          int cmax = valid - 1, cmin = -1, csink = 0;
-          if (!a.prefix && i >= tiles.ns) cmax = min(cmax, p - j0), cmin = wlo - j0, csink = a.sinks - j0;
-#pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (!(e <= cmax && (e >= cmin || e < csink))) v[e] = 0xff800000u;
-        }
-        float my = -INFINITY;
+      auto most = [&] {
+        float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
           my = max3(my, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
         }
-        mx = fmaxf(mx, my);
+        return fmaxf(mx, my);
+      };
+      // the load stands in both branches, so that the selects of one are not executed for the other
+      if (tiles.all(i)) {
+        tmem_ld32(sbase, v);
+        mx = most();
+      } else {
+        const int valid = tiles.valid(i) - 32 * half;
+        some = valid > 0;
+        if (some) {
+          tmem_ld32(sbase, v);
+          uint32_t see = low_bits(valid);  // of this thread's columns, those that its row sees
+          if (!a.prefix && i >= tiles.ns) {
+            const int j0 = tiles.first(i) + 32 * half;
+            see &= low_bits(p + 1 - j0) & (~low_bits(wlo - j0) | low_bits(a.sinks - j0));
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e++) v[e] = see >> e & 1 ? v[e] : 0xff800000u;
+          mx = most();
+        }
       }
       float(&exchange)[2][ROWS] = s_max[k & 1];
       exchange[half][row] = mx;
