@@ -9,11 +9,10 @@
 // fills the other's waits, its start and its end. In a CTA
 //   warp 0     TMA: K and V tiles into a ring each
 //   warp 1     TMEM and the MMAs: S = Q K^T, O += P V
-//   warps 2-9  the softmax
+//   warps 2-5  the softmax, one thread a row
 // S has two buffers: the next tile's scores are computed while this one's are in
-// the softmax. A row is shared by two threads, one for each half of its columns,
-// which exchange maxima through shared memory. The weights P take the place of S
-// in tensor memory and enter the second product from there.
+// the softmax. The weights P take the place of S in tensor memory and enter the
+// second product from there.
 // (Two tiles of rows and 128 positions with one S each, an SM to a CTA: the chain
 // softmax - P V - Q K^T took 4400 cycles for 128 positions of bf16, 128 values,
 // of which either unit was busy for half: 282 us for 8192 tokens, window 1500.)
@@ -46,7 +45,7 @@ namespace {
 using namespace dev;
 using namespace tc;
 
-constexpr int THREADS = 320, KT = 64, ROWS = 128;
+constexpr int THREADS = 192, KT = 64, ROWS = 128;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float GROWTH = 8.f;  // log2 of what a row may grow before its maximum is raised
 constexpr uint32_t COLS = 256, COL_O = 2 * KT;  // tensor memory: two buffers of S, then those of O
@@ -181,7 +180,6 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   // may wait for a product when the next one is done too.
   __shared__ uint64_t q_full, k_full[F::RING], v_full[F::RING], s_full[F::RING], o_full[F::RING], p_full[2];
   __shared__ uint32_t tmem_at;
-  __shared__ float s_max[2][2][ROWS];  // [tile parity][half][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
   const int r0 = (int)(gridDim.z - 1 - blockIdx.z) * ROWS;  // the longest rows first
@@ -191,14 +189,14 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   const int count = i1 - i0;
 
   if (tid == 0) {
-    mbar_init(&q_full, 8);
+    mbar_init(&q_full, 4);
     for (int i = 0; i < F::RING; i++) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&o_full[i], 1);
     }
-    for (int i = 0; i < 2; i++) mbar_init(&p_full[i], 8);
+    for (int i = 0; i < 2; i++) mbar_init(&p_full[i], 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&tmem_at, COLS);
@@ -291,14 +289,13 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     }
   } else {
     // -------------------------------------------------------------- softmax
-    const int half = ((warp - 2) >> 2) & 1, quarter = warp & 3, row = quarter * 32 + lane;  // TMEM lanes by warp % 4
+    const int quarter = warp & 3, row = quarter * 32 + lane;  // TMEM lanes by warp % 4
     const int R = r0 + min(row, nrows - 1), tok = R / a.g, head = kh * a.g + R % a.g;
     const bool live = row < nrows;
     {
       const Q* q = (const Q*)a.q + (size_t)tok * a.q_stride + (size_t)head * D;
 #pragma unroll
-      for (int i = 0; i < D / 16; i++) {
-        const int c = half * (D / 16) + i;
+      for (int c = 0; c < D / 8; c++) {
         uint8_t* chunk = smem + (c >> 3) * F::Q_CHUNK;
         if constexpr (PAIR) {
           const float4 u = *(const float4*)(q + 8 * c), v = *(const float4*)(q + 8 * c + 4);
@@ -321,13 +318,12 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       if (lane == 0) mbar_arrive(&q_full);
     }
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t obase = mine + COL_O + (D / 2) * half;
+    const uint32_t obase = mine + COL_O;
     const float sc = PAIR ? 1.f : a.scale2;
     const int p = a.start + tok;
     const int wlo = a.window > 0 ? p - a.window + 1 : -0x40000000;
-    const int pair = 1 + quarter;  // the named barrier of the two warps that share these rows
     float m = -INFINITY, l = 0.f, alpha_last = 0.f;
-    float o[PAIR ? D / 2 : 1] = {};  // fp32 queries: this half's columns of the running output
+    float o[PAIR ? D : 1] = {};  // fp32 queries: the running output
     bool ok = true;
     auto wait_o = [&](int k) {  // the k-th product has been added
       if (ok) ok = mbar_wait(&o_full[k % F::RING], (k / F::RING) & 1, nullptr);
@@ -339,55 +335,59 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
         __syncwarp();
 #pragma unroll
         for (int c = 0; c < D / 32; c++) {
-          uint32_t v[16];
-          tmem_ld16_nowait(obase + D * (k & (F::OBUF - 1)) + 16 * c, v);
-          tmem_wait_ld();
+          uint32_t v[32];
+          tmem_ld32(obase + D * (k & (F::OBUF - 1)) + 32 * c, v);
 #pragma unroll
-          for (int e = 0; e < 16; e++) o[16 * c + e] = fmaf(o[16 * c + e], alpha_last, __uint_as_float(v[e]));
+          for (int e = 0; e < 32; e++) o[32 * c + e] = fmaf(o[32 * c + e], alpha_last, __uint_as_float(v[e]));
         }
       }
     };
     for (int k = 0; k < count; k++) {
       const int i = i0 + k;
-      if (ok) ok = mbar_wait(&s_full[k % F::RING], (k / F::RING) & 1, nullptr);  // a warp that gave up still meets its partner below
+      if (ok) ok = mbar_wait(&s_full[k % F::RING], (k / F::RING) & 1, nullptr);
+      if (!ok) break;
       __syncwarp();
       tc_fence_after();
-      const uint32_t sbase = mine + KT * (k & 1) + 32 * half;
-      bool some = true;  // this half has columns
-      uint32_t v[32];
+      const uint32_t sbase = mine + KT * (k & 1);
+      bool upper = true;  // the tile has its second 32 columns
+      uint32_t v[2][32];
       float mx = -INFINITY;
-      auto most = [&] {
+      auto load = [&](int c) { tmem_ld32_nowait(sbase + 32 * c, v[c]); };
+      auto most = [&](int c) {
         float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          mx = max3(mx, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-          my = max3(my, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
+          mx = max3(mx, __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
+          my = max3(my, __uint_as_float(v[c][e + 2]), __uint_as_float(v[c][e + 3]));
         }
         return fmaxf(mx, my);
       };
-      // the load stands in both branches, so that the selects of one are not executed for the other
+      // the loads stand in both branches, so that the selects of one are not executed for the other
       if (tiles.all(i)) {
-        tmem_ld32(sbase, v);
-        mx = most();
+        load(0);
+        load(1);
+        tmem_wait_ld();
+        mx = fmaxf(most(0), most(1));
       } else {
-        const int valid = tiles.valid(i) - 32 * half;
-        some = valid > 0;
-        if (some) {
-          tmem_ld32(sbase, v);
-          uint32_t see = low_bits(valid);  // of this thread's columns, those that its row sees
-          if (!a.prefix && i >= tiles.ns) {
-            const int j0 = tiles.first(i) + 32 * half;
-            see &= low_bits(p + 1 - j0) & (~low_bits(wlo - j0) | low_bits(a.sinks - j0));
-          }
+        const int valid = tiles.valid(i);
+        upper = valid > 32;
+        load(0);
+        if (upper) load(1);
+        tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e++) v[e] = see >> e & 1 ? v[e] : 0xff800000u;
-          mx = most();
-        }
+        for (int c = 0; c < 2; c++)
+          if (c == 0 || upper) {
+            uint32_t see = low_bits(valid - 32 * c);  // of these columns, those that the row sees
+            if (!a.prefix && i >= tiles.ns) {
+              const int j0 = tiles.first(i) + 32 * c;
+              see &= low_bits(p + 1 - j0) & (~low_bits(wlo - j0) | low_bits(a.sinks - j0));
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e++) v[c][e] = see >> e & 1 ? v[c][e] : 0xff800000u;
+            mx = fmaxf(mx, most(c));
+          }
       }
-      float(&exchange)[2][ROWS] = s_max[k & 1];
-      exchange[half][row] = mx;
-      asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-      mx = fmaxf(mx, exchange[half ^ 1][row]) * sc;
+      mx *= sc;
       float alpha = 1.f;
       if (PAIR || __any_sync(0xffffffffu, mx > m + GROWTH)) {
         const float mn = fmaxf(m, mx);
@@ -397,39 +397,41 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           __syncwarp();
 #pragma unroll
           for (int c = 0; c < D / 32; c++) {
-            uint32_t w[16];
-            tmem_ld16_nowait(obase + 16 * c, w);
-            tmem_wait_ld();
+            uint32_t w[32];
+            tmem_ld32(obase + 32 * c, w);
 #pragma unroll
-            for (int e = 0; e < 16; e++) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
-            tmem_st16(obase + 16 * c, w);
+            for (int e = 0; e < 32; e++) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
+            tmem_st16(obase + 32 * c, w);
+            tmem_st16(obase + 32 * c + 16, w + 16);
           }
         }
         l *= alpha;
         m = mn;
       }
       if (F::OBUF == 1 && k > 0) fold(k - 1);
-      if (some) {
-        const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: its weights are all 0
-        const uint64_t sc2 = two(sc, sc), ms2 = two(-ms, -ms);
-        uint64_t la = 0, lb = 0;  // pairs of 0.f
-        uint32_t hi[16], lo[16];
+      const float ms = m == -INFINITY ? 0.f : m;  // a row that has seen nothing yet: its weights are all 0
+      const uint64_t sc2 = two(sc, sc), ms2 = two(-ms, -ms);
+      uint64_t la = 0, lb = 0;  // pairs of 0.f
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          const float2 z = one(fma2(two(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, ms2));
-          const float u = exp2_fast(z.x), w = exp2_fast(z.y);
-          if (e & 1)
-            lb = add2(lb, two(u, w));
-          else
-            la = add2(la, two(u, w));
-          hi[e] = pack(C(), u, w);
-          if constexpr (PAIR) lo[e] = rest(hi[e], u, w);
+      for (int c = 0; c < 2; c++)
+        if (c == 0 || upper) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int e = 0; e < 16; e++) {
+            const float2 z = one(fma2(two(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), sc2, ms2));
+            const float u = exp2_fast(z.x), w = exp2_fast(z.y);
+            if (e & 1)
+              lb = add2(lb, two(u, w));
+            else
+              la = add2(la, two(u, w));
+            hi[e] = pack(C(), u, w);
+            if constexpr (PAIR) lo[e] = rest(hi[e], u, w);
+          }
+          tmem_st16(sbase + 32 * c, hi);
+          if constexpr (PAIR) tmem_st16(sbase + 32 * c + 16, lo);
         }
-        tmem_st16(sbase, hi);
-        if constexpr (PAIR) tmem_st16(sbase + 16, lo);
-        const float2 sum = one(add2(la, lb));
-        l += sum.x + sum.y;
-      }
+      const float2 sum = one(add2(la, lb));
+      l += sum.x + sum.y;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -446,16 +448,12 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     }
     if (!ok && lane == 0) report(BAD_WAIT);
     // ------------------------------------------------------------ epilogue
-    // the partner has read the last tile's maxima: the product it took part in is done
-    s_max[0][half][row] = l;
     if (nranks == 1) {
-      asm volatile("bar.sync %0, 64;" ::"r"(pair) : "memory");
-      l += s_max[0][half ^ 1][row];
       const float inv = l == 0.f && m == -INFINITY ? 0.f : 1.f / l;
       const size_t at = (size_t)kh * a.rows + R;
       if (has) {
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) {
+        for (int c = 0; c < D / 32; c++) {
           uint32_t v[32];
           __syncwarp();
           if constexpr (PAIR) {
@@ -464,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           } else {
             tmem_ld32(obase + 32 * c, v);
           }
-          const int col = (D / 2) * half + 32 * c;
+          const int col = 32 * c;
           if (live) {
             if (a.prefix)
               store_row<float>(a.part + at * D + col, v, 1.f);
@@ -472,7 +470,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
               store_row<Q>((Q*)a.out + (size_t)tok * a.out_stride + (size_t)head * D + col, v, inv);
           }
         }
-        if (live && half == 0) {
+        if (live) {
           if (a.prefix)
             a.part_ml[at] = make_float2(m, l);
           else if (a.lse)
@@ -481,23 +479,20 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       }
     } else {
       // every CTA of the cluster is past its ring and its queries: row r goes to CTA r % nranks, behind the parts of lower ranks
-      asm volatile("bar.sync 9, 256;" ::: "memory");
-      l += s_max[0][half ^ 1][row];
+      asm volatile("bar.sync 1, 128;" ::: "memory");
       asm volatile("barrier.cluster.wait.acquire;\nbarrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
       const int each = (ROWS + nranks - 1) / nranks;  // rows of a CTA
       float* so = (float*)smem;
       float2* s_ml = (float2*)(smem + ROWS * F::STRIDE * 4);
       const int at = rank * each + row / nranks;
       if (row < nrows) {
-        if (half == 0) {
-          const uint32_t ml_at = peer(&s_ml[at], row % nranks);
-          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(ml_at), "f"(has ? m : -INFINITY), "f"(has ? l : 0.f)
-                       : "memory");
-        }
+        const uint32_t ml_at = peer(&s_ml[at], row % nranks);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(ml_at), "f"(has ? m : -INFINITY), "f"(has ? l : 0.f)
+                     : "memory");
       }
       if (has) {
 #pragma unroll
-        for (int c = 0; c < D / 64; c++) {
+        for (int c = 0; c < D / 32; c++) {
           uint32_t v[32];
           __syncwarp();
           if constexpr (PAIR) {
@@ -507,7 +502,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
             tmem_ld32(obase + 32 * c, v);
           }
           if (row < nrows) {
-            const uint32_t to = peer(&so[at * F::STRIDE + (D / 2) * half + 32 * c], row % nranks);
+            const uint32_t to = peer(&so[at * F::STRIDE + 32 * c], row % nranks);
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + 4 * e), "r"(v[e]), "r"(v[e + 1]),
@@ -521,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       // this CTA's rows, 4 columns to a thread
       constexpr int PER = D / 4;
       const int c = tid % PER * 4;
-      for (int k = (tid - 64) / PER; k * nranks + rank < nrows; k += 256 / PER) {
+      for (int k = (tid - 64) / PER; k * nranks + rank < nrows; k += 128 / PER) {
         float M = -INFINITY, L = 0.f;
         float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int y = 0; y < nranks; y++) M = fmaxf(M, s_ml[y * each + k].x);
