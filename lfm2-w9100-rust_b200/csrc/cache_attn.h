@@ -71,6 +71,7 @@ cudaError_t shared(const Decode& a, cudaStream_t s);
 cudaError_t evict(const Evict& a, cudaStream_t s);
 // Adds what the kernels of each file have reported on this device to *bits and clears it; waits for the stream.
 cudaError_t take_status_tc(unsigned* bits, cudaStream_t s);
+cudaError_t take_status_weights(unsigned* bits, cudaStream_t s);
 cudaError_t take_status_decode(unsigned* bits, cudaStream_t s);
 cudaError_t take_status_evict(unsigned* bits, cudaStream_t s);
 

@@ -231,6 +231,7 @@ lfm_status lfm_attention_status(uint32_t* status, void* stream) {
   if (!status) return bad(who, "status is null");
   unsigned bits = 0;
   cudaError_t e = lfm::cache::take_status_tc(&bits, (cudaStream_t)stream);
+  if (e == cudaSuccess) e = lfm::cache::take_status_weights(&bits, (cudaStream_t)stream);
   if (e == cudaSuccess) e = lfm::cache::take_status_decode(&bits, (cudaStream_t)stream);
   if (e == cudaSuccess) e = lfm::cache::take_status_evict(&bits, (cudaStream_t)stream);
   *status = bits;

@@ -34,10 +34,8 @@
 #include <mutex>
 #include <type_traits>
 
-#include "cache_attn.h"
-#include "cache_common.cuh"
+#include "cache_tc.cuh"
 #include "host_once.h"
-#include "tc_common.cuh"
 
 namespace lfm {
 namespace cache {
@@ -82,63 +80,6 @@ struct Rows {
   float* part;     // prefix: O [kv head][row][D], not divided
   float2* part_ml; // prefix: (m in log2 units, l)
 };
-
-// The MMAs are issued by one elected lane of a converged warp: with the branch
-// around the instruction alone, addresses and descriptors stay in uniform
-// registers (under a branch around the whole loop an MMA took ~100 cycles to
-// issue and 64 to run).
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(db), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile(
-      "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
-      : "memory");
-}
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(at),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t pack(__half, float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *(const uint32_t*)&h;
-}
-__device__ __forceinline__ uint32_t pack(__nv_bfloat16, float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *(const uint32_t*)&h;
-}
-// what an fp16 pair leaves off, as the next fp16 pair
-__device__ __forceinline__ uint32_t rest(uint32_t hi, float a, float b) {
-  const float2 back = __half22float2(*(const __half2*)&hi);
-  return pack(__half(), a - back.x, b - back.y);
-}
-// 16 bytes at column block `piece` (of 8) of row r of a swizzled 64-wide chunk
-__device__ __forceinline__ void st_piece(uint8_t* chunk, int r, int piece, uint4 v) {
-  *(uint4*)(chunk + r * 128 + ((piece ^ (r & 7)) << 4)) = v;
-}
-
-// The n lowest bits.
-__device__ __forceinline__ uint32_t low_bits(int n) {
-  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
-}
 
 // The position tiles of a block of rows: the sinks in front of the window, then
 // the positions from the first row's window to the last row. A tile has `width`
@@ -558,34 +499,6 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   }
 }
 
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return (EncodeFn)p;
-  }();
-  return fn;
-}
-
-// A cache slot [kv head][position][d] of 16-bit values, read in boxes of 64 values x 64 positions of one head.
-cudaError_t map_cache(CUtensorMap* map, const void* base, int kv_heads, int ctx, int d) {
-  EncodeFn fn = encode_fn();
-  if (!fn) return cudaErrorNotSupported;
-  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)ctx, (cuuint64_t)kv_heads};
-  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)ctx * d * 2};
-  const cuuint32_t box[3] = {64, KT, 1}, step[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, step,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
-
 // CTAs that split one block's positions: as many as fill the SMs, each with a tile of its own at least.
 int split(int blocks, int tiles) {
   int n = 1;
@@ -597,8 +510,8 @@ template <int T, int D>
 cudaError_t launch(const Rows& a, const void* k, const void* v, int ctx, int tiles, cudaStream_t s) {
   using F = Cfg<T, D>;
   CUtensorMap mk, mv;
-  cudaError_t e = map_cache(&mk, k, a.kv_heads, ctx, D);
-  if (e == cudaSuccess) e = map_cache(&mv, v, a.kv_heads, ctx, D);
+  cudaError_t e = map_cache(&mk, k, a.kv_heads, ctx, D, KT);
+  if (e == cudaSuccess) e = map_cache(&mv, v, a.kv_heads, ctx, D, KT);
   if (e != cudaSuccess) return e;
   auto* f = k_rows<T, D>;
   static unsigned long long done = 0;
