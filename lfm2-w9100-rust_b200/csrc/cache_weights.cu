@@ -9,14 +9,14 @@
 // heads of a KV head, token by token) at a time:
 //   warp 0      16-bit queries: the tiles by TMA
 //   warp 1      TMEM and the MMAs, into two buffers of S^T
-//   warps 2-9   the sums; a key is shared by two threads, one for each half of the columns
-//   from 10 on  the rows' lse, and for fp32 queries the tiles: fp16 hi/lo pairs,
-//               two MMAs (eight warps, one for 16-bit queries)
-// Bound by the exponentials: the special-function unit takes 8 cycles for a
-// warp's 32, more than all other instructions of a term together. So of every 16
-// pairs of terms EMULATED go through the fma units instead (Cody and Waite's range
-// reduction, x = n + f with |f| <= 1/2, and a minimax polynomial of 2^f, fitted
-// for the relative error, 1e-7), until both units are busy for as long.
+//   warps 2-17  the sums; a key is shared by four threads, each for a quarter of the columns
+//   from 18 on  the rows' lse, and for fp32 queries the tiles: fp16 hi/lo pairs, two MMAs
+// Bound by the exponentials: 16 a cycle and SM, 2048 cycles for a tile of 128
+// keys and 256 rows. 8191 bf16 tokens of 32 heads and 128 values: 336 us, the special-function units
+// busy for 80% of it. A third of the exponentials through the fma units (range
+// reduction and a polynomial of degree 5) took the units' time down to 55% and left the total
+// (341 us): the issuing warp and the sums' start on each tile are what is left. Tiles of 128 rows
+// in four buffers: 350 us; eight warps for the sums: 434 us.
 // A key is summed by one thread, in the order of the rows, tile by tile, and the
 // CTAs of a cluster that splits the rows are added up in their order: the
 // result is the same on every run.
@@ -31,15 +31,14 @@ namespace lfm {
 namespace cache {
 namespace {
 
-constexpr int KEYS = 128, EPI = 8, LSE_RING = 4;
+constexpr int KEYS = 128, EPI = 16, PARTS = EPI / 4, LSE_RING = 4;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int EMULATED = 5;  // of 16 pairs of terms
 
 template <int T, int D>
 struct Cfg {
   static constexpr bool PAIR = T == T_F32;
   static constexpr int N = PAIR && D == 128 ? 128 : 256;  // rows of a tile at most: two tiles have to fit
-  static constexpr int FEED = PAIR ? 8 : 1;               // warps that write lse, and fp32 queries
+  static constexpr int FEED = PAIR ? 4 : 2;  // warps that write lse, and fp32 queries
   static constexpr int THREADS = 32 * (2 + EPI + FEED);
   static constexpr int K_CHUNK = KEYS * 128, K_TILE = K_CHUNK * (D / 64);
   static constexpr int Q_CHUNK = N * 128, Q_TILE = Q_CHUNK * (D / 64), STAGE = (PAIR ? 2 : 1) * Q_TILE;
@@ -59,22 +58,6 @@ struct Args {
   float* acc;
 };
 
-// 2^x for two values by fma instructions. Below 2^-126 the result is 2^-126.
-__device__ __forceinline__ uint64_t exp2_fma(float2 x) {
-  const uint64_t v = two(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const uint64_t magic = two(12582912.f, 12582912.f), minus = two(-12582912.f, -12582912.f);  // 1.5 * 2^23: rounds to an integer
-  const uint64_t t = add2(v, magic);
-  const uint64_t f = fma2(add2(t, minus), two(-1.f, -1.f), v);
-  uint64_t p = fma2(two(0.0013276472f, 0.0013276472f), f, two(0.009675541f, 0.009675541f));
-  p = fma2(p, f, two(0.05550713f, 0.05550713f));
-  p = fma2(p, f, two(0.2402212f, 0.2402212f));
-  p = fma2(p, f, two(0.69314694f, 0.69314694f));
-  p = fma2(p, f, two(1.0000001f, 1.0000001f));
-  const float2 r = one(p), n = one(t);
-  return two(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)),
-             __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
-}
-
 template <int T, int D>
 __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
     k_weights(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q, const Args a) {
@@ -85,8 +68,8 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
   extern __shared__ __align__(1024) uint8_t smem[];  // K, then the ring of query tiles
   __shared__ uint64_t k_full, full[F::RING], empty[F::RING], s_full[2], s_free[2], lse_full[LSE_RING], lse_free[LSE_RING];
   __shared__ uint32_t tmem_at;
-  __shared__ __align__(16) float s_lse[LSE_RING][256];  // -lse in log2 units
-  __shared__ float s_sum[8][KEYS];                      // half sums, then those of the cluster's CTAs
+  __shared__ __align__(16) float s_lse[LSE_RING][F::N];  // -lse in log2 units
+  __shared__ float s_sum[8][KEYS];                      // the quarters' sums, then those of the cluster's CTAs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
   const int j0 = blockIdx.z * KEYS;  // the first keys, which most rows see, come first
@@ -169,7 +152,8 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
     }
   } else if (warp < 2 + EPI) {
     // --------------------------------------------------------------- sums
-    const int half = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane, j = j0 + key;
+    constexpr int COLS = F::N / PARTS;
+    const int part = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane, j = j0 + key;
     const float sc = PAIR ? 1.f : a.scale2;
     const uint64_t sc2 = two(sc, sc);
     for (int k = 0; k < count; k++) {
@@ -188,24 +172,22 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
         hi = min(a.tokens, a.n - t0) * a.g;
         if (a.window && j >= a.sinks) hi = min(hi, max(0, j + a.window - p0) * a.g);
       }
-      const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + 256 * (k & 1) + half * (F::N / 2);
-      const float* nl = s_lse[k % LSE_RING] + half * (F::N / 2);
+      const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + 256 * (k & 1) + part * COLS;
+      const float* nl = s_lse[k % LSE_RING] + part * COLS;
       uint64_t s2[2] = {0, 0};  // pairs of 0.f
-      uint32_t v[2][32];
-      tmem_ld32_nowait(at, v[0]);
 #pragma unroll
-      for (int c = 0; c < F::N / 64; c++) {
-        tmem_wait_ld();
-        if (c + 1 < F::N / 64) tmem_ld32_nowait(at + 32 * (c + 1), v[(c + 1) & 1]);
-        uint32_t(&w)[32] = v[c & 1];
-        const int c0 = half * (F::N / 2) + 32 * c;
-        const uint32_t see = low_bits(hi - c0) & ~low_bits(lo - c0);
-        if (__all_sync(0xffffffffu, see == 0)) continue;
-        if (__any_sync(0xffffffffu, see != 0xffffffffu)) {
+      for (int c = 0; c < COLS / 32; c++) {
+        uint32_t w[32];
+        tmem_ld32(at + 32 * c, w);
+        const int c0 = part * COLS + 32 * c;
+        if (!all || c0 + 32 > cols) {
+          const uint32_t see = low_bits(hi - c0) & ~low_bits(lo - c0);
+          if (__any_sync(0xffffffffu, see != 0)) {
 #pragma unroll
-          for (int e = 0; e < 32; e++) {
-            const float x = exp2_fast(fmaf(__uint_as_float(w[e]), sc, nl[32 * c + e]));
-            if (see >> e & 1) sum += x;
+            for (int e = 0; e < 32; e++) {
+              const float x = exp2_fast(fmaf(__uint_as_float(w[e]), sc, nl[32 * c + e]));
+              if (see >> e & 1) sum += x;
+            }
           }
           continue;
         }
@@ -215,11 +197,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
           const uint64_t x = fma2(two(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1])), sc2,
                                   e & 1 ? two(n4.z, n4.w) : two(n4.x, n4.y));
           const float2 y = one(x);
-          // spread over the 16: e * EMULATED / 16 steps up EMULATED times
-          if ((e + 1) * EMULATED / 16 != e * EMULATED / 16)
-            s2[e & 1] = add2(s2[e & 1], exp2_fma(y));
-          else
-            s2[e & 1] = add2(s2[e & 1], two(exp2_fast(y.x), exp2_fast(y.y)));
+          s2[e & 1] = add2(s2[e & 1], two(exp2_fast(y.x), exp2_fast(y.y)));
         }
       }
       tc_fence_before();
@@ -231,19 +209,38 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
       const float2 s = one(add2(s2[0], s2[1]));
       sum += s.x + s.y;
     }
-    s_sum[half][key] = sum;
+    s_sum[part][key] = sum;
   } else {
     // ---------------------------------------------------------- lse, fp32 queries
     const int ft = tid - 32 * (2 + EPI);
-    for (int k = 0; k < count; k++) {
-      const int st = k % F::RING, t0 = (i0 + k) * a.tokens;
-      if (k >= LSE_RING && !(ok = mbar_wait(&lse_free[k % LSE_RING], (k / LSE_RING - 1) & 1, nullptr))) break;
-      const int have = min(a.tokens, a.n - t0) * a.g;  // rows that exist
-      for (int c = ft; c < F::N; c += 32 * F::FEED)
-        s_lse[k % LSE_RING][c] =
-            c < have ? -LOG2E * a.lse[(size_t)(t0 + c / a.g) * a.heads + kh * a.g + c % a.g] : -INFINITY;
+    constexpr int PER = (F::N + 32 * F::FEED - 1) / (32 * F::FEED), AHEAD = 4;
+    float pre[AHEAD][PER];  // loaded AHEAD tiles before they are stored: under the tiles' traffic a load takes ~2700 cycles
+    int off[PER];           // of a row's lse from that of its tile's first token
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int c = ft + 32 * F::FEED * i;
+      off[i] = c / a.g * a.heads + c % a.g;
+    }
+    auto fetch = [&](int k, float(&e)[PER]) {
+      const int t0 = (i0 + k) * a.tokens, have = min(a.tokens, a.n - t0) * a.g;  // rows that exist
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const int c = ft + 32 * F::FEED * i;
+        e[i] = INFINITY;
+        if (k < count && c < have) e[i] = a.lse[(size_t)t0 * a.heads + kh * a.g + off[i]];
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) fetch(i, pre[i]);
+    auto feed = [&](int k, float(&e)[PER]) {
+      const int st = k % F::RING, t0 = (i0 + k) * a.tokens, have = min(a.tokens, a.n - t0) * a.g;
+      if (k >= LSE_RING && !(ok = mbar_wait(&lse_free[k % LSE_RING], (k / LSE_RING - 1) & 1, nullptr))) return;
+#pragma unroll
+      for (int i = 0; i < PER; i++)
+        if (ft + 32 * F::FEED * i < F::N) s_lse[k % LSE_RING][ft + 32 * F::FEED * i] = -LOG2E * e[i];
+      fetch(k + AHEAD, e);
       if constexpr (PAIR) {
-        if (k >= F::RING && !(ok = mbar_wait(&empty[st], (k / F::RING - 1) & 1, nullptr))) break;
+        if (k >= F::RING && !(ok = mbar_wait(&empty[st], (k / F::RING - 1) & 1, nullptr))) return;
         uint8_t* dst = smem + F::K_TILE + st * F::STAGE;
 #pragma unroll 4
         for (int i = ft; i < cols * (D / 8); i += 32 * F::FEED) {
@@ -272,7 +269,11 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
         mbar_arrive(&lse_full[k % LSE_RING]);
         if (PAIR) mbar_arrive(&full[st]);
       }
-    }
+    };
+    for (int k = 0; k < count && ok; k += AHEAD)
+#pragma unroll
+      for (int i = 0; i < AHEAD; i++)
+        if (k + i < count && ok) feed(k + i, pre[i]);
   }
   if (!ok && lane == 0) report(BAD_WAIT);
   tc_fence_before();
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-  if (tid < KEYS) sum = s_sum[0][tid] + s_sum[1][tid];
+  if (tid < KEYS) sum = (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
   if (nranks > 1) {
     // to the first CTA, which adds them up in the order of the ranks
     __syncthreads();
