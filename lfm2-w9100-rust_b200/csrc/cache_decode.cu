@@ -20,8 +20,8 @@
 //       permutes; output column n of tile e is head_dim index 8 n + e.
 // Statistics and outputs stay in fp32; exponentials are of powers of two (the
 // queries or the scores carry scale * log2 e). The warps join through shared
-// memory, the CTAs through the cluster's, each CTA finishing a share of the
-// columns, so a call is one launch without workspace. Accumulated weights need
+// memory, the CTAs through the cluster's: each sends its part of the columns to
+// the CTA that finishes them, so a call is one launch without workspace. Accumulated weights need
 // the joined statistics: a CTA keeps its scores in shared memory until the
 // join, or, where they would not fit, reads K once more.
 #include <algorithm>
@@ -37,7 +37,7 @@ namespace cache {
 namespace {
 using namespace dev;
 
-constexpr int WARPS = 4, STAGES = 3, HALF = 4096, STAGE = 2 * HALF;
+constexpr int WARPS = 4, STAGES = 2, HALF = 4096, STAGE = 2 * HALF;
 constexpr int RING = WARPS * STAGES * STAGE;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int SCORE_BYTES = 96 * 1024;  // most that a CTA keeps of its scores
@@ -74,8 +74,9 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
   extern __shared__ __align__(1024) uint8_t smem[];
   float* scores = (float*)(smem + RING);  // STORED: [head][cap]
   __shared__ uint64_t full[WARPS][STAGES];
-  __shared__ __align__(16) float s_o[8][D];
-  __shared__ float s_m[8], s_l[8], w_m[WARPS][8], w_l[WARPS][8], f_m[8], f_inv[8], f_pre[8];
+  __shared__ __align__(16) float4 s_o[8 * D / 4 + 16];  // this CTA's share of the columns, from every CTA: [CTA][item]
+  __shared__ float2 s_ml[16][8];                   // every CTA's statistics
+  __shared__ float w_m[WARPS][8], w_l[WARPS][8], f_m[8], f_inv[8], f_pre[8];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
   const int g = a.heads / a.kv_heads;
@@ -90,6 +91,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
   const size_t base = (size_t)slot * a.slot_stride + (size_t)kh * a.ctx * D;
   const C *kg = (const C*)a.k + base, *vg = (const C*)a.v + base;
   uint8_t* ring = smem + w * STAGES * STAGE;
+  if (nranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   if (lane < STAGES) mbar_init(&full[w][lane], 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -270,56 +272,65 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
     }
   if (!ok && lane == 0) report(BAD_WAIT);
   __syncthreads();
-  for (int i = tid; i < 8 * D / 4; i += WARPS * 32) {
+  // join the CTAs: item i (head, 4 columns) goes to CTA i % nranks, the statistics to all
+  if (nranks > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // they have started
+  const int items = g * (D / 4), share = (items + nranks - 1) / nranks;
+  for (int i = tid; i < items; i += WARPS * 32) {
     const int h = i / (D / 4);
     float M = -INFINITY;
 #pragma unroll
     for (int x = 0; x < WARPS; x++) M = fmaxf(M, w_m[x][h]);
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
 #pragma unroll
     for (int x = 0; x < WARPS; x++) {
       const float c = part_weight(w_m[x][h], M);
       const float4 y = ((const float4*)(smem + x * STAGES * STAGE))[i];
       f.x = fmaf(c, y.x, f.x), f.y = fmaf(c, y.y, f.y), f.z = fmaf(c, y.z, f.z), f.w = fmaf(c, y.w, f.w);
-      L = fmaf(c, w_l[x][h], L);
     }
-    ((float4*)s_o)[i] = f;
-    if (i % (D / 4) == 0) {
-      s_m[h] = M;
-      s_l[h] = L;
-    }
+    if (nranks == 1)
+      s_o[i] = f;
+    else
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(peer(&s_o[rank * share + i / nranks], i % nranks)),
+                   "f"(f.x), "f"(f.y), "f"(f.z), "f"(f.w)
+                   : "memory");
   }
-  if (nranks > 1)
+  for (int i = tid; i < g * nranks; i += WARPS * 32) {
+    const int h = i % g;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int x = 0; x < WARPS; x++) M = fmaxf(M, w_m[x][h]);
+#pragma unroll
+    for (int x = 0; x < WARPS; x++) L = fmaf(part_weight(w_m[x][h], M), w_l[x][h], L);
+    asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer(&s_ml[rank][h], i / g)), "f"(M), "f"(L) : "memory");
+  }
+  if (nranks > 1) {
+    __syncwarp();
     cluster_sync();
-  else
+  } else {
     __syncthreads();
-
-  // join the CTAs and the prefix's parts: the joint statistics of each head, then this CTA's share of the columns
+  }
   if (pre.o) pdl_wait();
   const size_t row0 = ((size_t)kh * a.batch + b) * g;  // of the prefix's part
   if (tid < g) {
     float M = -INFINITY, L = 0.f;
-    for (int x = 0; x < nranks; x++) M = fmaxf(M, ld_peer(peer(&s_m[tid], x)));
     float2 ml = make_float2(-INFINITY, 0.f);
     if (pre.o) ml = pre.ml[row0 + tid];
+    for (int x = 0; x < nranks; x++) M = fmaxf(M, s_ml[x][tid].x);
     M = fmaxf(M, ml.x);
-    for (int x = 0; x < nranks; x++)
-      L = fmaf(part_weight(ld_peer(peer(&s_m[tid], x)), M), ld_peer(peer(&s_l[tid], x)), L);
+    for (int x = 0; x < nranks; x++) L = fmaf(part_weight(s_ml[x][tid].x, M), s_ml[x][tid].y, L);
     L = fmaf(part_weight(ml.x, M), ml.y, L);
     f_pre[tid] = part_weight(ml.x, M);
     f_m[tid] = M;
     f_inv[tid] = M == -INFINITY && L == 0.f ? 0.f : 1.f / L;  // nothing seen: zeros
   }
   __syncthreads();
-  const int items = g * (D / 4);
-  for (int i = tid * nranks + rank; i < items; i += WARPS * 32 * nranks) {
-    const int h = i / (D / 4), c = i % (D / 4) * 4;
+  for (int k = tid; k * nranks + rank < items; k += WARPS * 32) {
+    const int i = k * nranks + rank, h = i / (D / 4), c = i % (D / 4) * 4;
     const float M = f_m[h], inv = f_inv[h];
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int x = 0; x < nranks; x++) {
-      const float wt = part_weight(ld_peer(peer(&s_m[h], x)), M);
-      const float4 y = ld_peer4(peer(&s_o[h][c], x));
+      const float wt = part_weight(s_ml[x][h].x, M);
+      const float4 y = s_o[x * share + k];
       f.x = fmaf(wt, y.x, f.x), f.y = fmaf(wt, y.y, f.y), f.z = fmaf(wt, y.z, f.z), f.w = fmaf(wt, y.w, f.w);
     }
     if (pre.o) {
@@ -327,11 +338,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
       const float4 y = *(const float4*)(pre.o + (row0 + h) * D + c);
       f.x = fmaf(wt, y.x, f.x), f.y = fmaf(wt, y.y, f.y), f.z = fmaf(wt, y.z, f.z), f.w = fmaf(wt, y.w, f.w);
     }
-    Q* dst = (Q*)a.out + (size_t)b * a.out_stride + (size_t)(kh * g + h) * D + c;
-    from_f32(good ? f.x * inv : 0.f, dst);
-    from_f32(good ? f.y * inv : 0.f, dst + 1);
-    from_f32(good ? f.z * inv : 0.f, dst + 2);
-    from_f32(good ? f.w * inv : 0.f, dst + 3);
+    store4((Q*)a.out + (size_t)b * a.out_stride + (size_t)(kh * g + h) * D + c,
+           good ? make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
   }
   if constexpr (ACC != NO_ACC) {
     if (good) {
@@ -374,7 +382,6 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
       }
     }
   }
-  if (nranks > 1) cluster_sync();  // the peers have read this CTA's part
 }
 
 template <int T, int D, int ACC>
@@ -407,7 +414,7 @@ cudaError_t run(const Decode& a, const Joint& pre, cudaStream_t s) {
   const long long most = a.window ? std::min<long long>(a.max_len, (long long)a.window + a.sinks) : a.max_len;
   const int chunks = (int)((most + kc - 1) / kc);
   int nranks = 1;
-  while (nranks < 16 && (long long)a.batch * a.kv_heads * nranks < 4 * 148 && chunks > WARPS * nranks) nranks *= 2;
+  while (nranks < 16 && (long long)a.batch * a.kv_heads * nranks < 3 * 148 && chunks > WARPS * nranks) nranks *= 2;
   // the most positions that one CTA may get, padded to whole chunks
   const int cap = ((chunks + nranks - 1) / nranks) * kc;
   const int acc = !a.acc ? NO_ACC : (long long)cap * (a.heads / a.kv_heads) * 4 <= SCORE_BYTES ? STORED : AGAIN;
