@@ -2,7 +2,7 @@
 // own-cache half of lfm_attention_shared with the join of both halves.
 //
 // A cluster of C CTAs takes one KV head of one session and splits the positions
-// that its query sees; each of a CTA's 4 warps walks its own chunks of 4 KB of
+// that its query sees; each of a CTA's warps walks its own chunks of 4 KB of
 // K and 4 KB of V (32 positions of 64 values, 16 of 128). A chunk's rows lie
 // one behind the other in memory, so a warp's lane 0 fetches it with one bulk
 // copy each (two where it spans the end of the sinks) into the warp's private
@@ -37,11 +37,14 @@ namespace cache {
 namespace {
 using namespace dev;
 
-constexpr int WARPS = 4, STAGES = 2, HALF = 4096, STAGE = 2 * HALF;
-constexpr int RING = WARPS * STAGES * STAGE;
+constexpr int STAGES = 2, HALF = 4096, STAGE = 2 * HALF;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int SCORE_BYTES = 96 * 1024;  // most that a CTA keeps of its scores
 enum Acc { NO_ACC = 0, STORED = 1, AGAIN = 2 };
+// Three CTAs of 4 warps to an SM; where the scores are kept, one of 7 warps with what its ring leaves of shared memory
+// (24 sessions of up to 32768 positions, 6 heads of 128 values to a KV head: 288 us without weights).
+constexpr int warps_of(int acc) { return acc == STORED ? 7 : 4; }
+constexpr int ring_of(int acc) { return warps_of(acc) * STAGES * STAGE; }
+constexpr int SCORE_BYTES = 227 * 1024 - ring_of(STORED) - 6 * 1024;
 
 template <class C>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -66,16 +69,17 @@ struct Joint {
 };
 
 template <int T, int D, int ACC>
-__global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int cap) {
+__global__ void __launch_bounds__(warps_of(ACC) * 32) k_decode(Decode a, Joint pre, int cap) {
   using Q = typename Types<T>::Q;
   using C = typename Types<T>::C;
+  constexpr int WARPS = warps_of(ACC), RING = ring_of(ACC);
   constexpr int KC = HALF / (2 * D);  // positions of a chunk
   constexpr int NU = D / 64, TILES = KC / 8;
   extern __shared__ __align__(1024) uint8_t smem[];
   float* scores = (float*)(smem + RING);  // STORED: [head][cap]
   __shared__ uint64_t full[WARPS][STAGES];
   __shared__ __align__(16) float4 s_o[8 * D / 4 + 16];  // this CTA's share of the columns, from every CTA: [CTA][item]
-  __shared__ float2 s_ml[16][8];                   // every CTA's statistics
+  __shared__ float2 s_ml[8][8];                    // every CTA's statistics
   __shared__ float w_m[WARPS][8], w_l[WARPS][8], f_m[8], f_inv[8], f_pre[8];
   const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
@@ -386,17 +390,16 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
 
 template <int T, int D, int ACC>
 cudaError_t launch(const Decode& a, const Joint& pre, int nranks, int cap, cudaStream_t s) {
-  const int smem = RING + (ACC == STORED ? a.heads / a.kv_heads * cap * 4 : 0);
+  const int smem = ring_of(ACC) + (ACC == STORED ? a.heads / a.kv_heads * cap * 4 : 0);
   auto* f = k_decode<T, D, ACC>;
   static unsigned long long done = 0;
   static std::mutex mu;
   once_per_device(done, mu, [f] {
-    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, RING + (ACC == STORED ? SCORE_BYTES : 0));
-    cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_of(ACC) + (ACC == STORED ? SCORE_BYTES : 0));
   });
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(nranks, a.kv_heads, a.batch);
-  c.blockDim = dim3(WARPS * 32);
+  c.blockDim = dim3(warps_of(ACC) * 32);
   c.dynamicSmemBytes = smem;
   c.stream = s;
   cudaLaunchAttribute at[2];
@@ -413,16 +416,21 @@ cudaError_t run(const Decode& a, const Joint& pre, cudaStream_t s) {
   const int kc = HALF / (2 * a.d);
   const long long most = a.window ? std::min<long long>(a.max_len, (long long)a.window + a.sinks) : a.max_len;
   const int chunks = (int)((most + kc - 1) / kc);
+  // As many CTAs to a KV head as fill three to an SM, each with chunks for its warps; more where that lets the scores
+  // be kept. At most 8: clusters of 16 left most SMs without a second CTA (625 us for the case above).
+  const int g = a.heads / a.kv_heads;
   int nranks = 1;
-  while (nranks < 16 && (long long)a.batch * a.kv_heads * nranks < 3 * 148 && chunks > WARPS * nranks) nranks *= 2;
-  // the most positions that one CTA may get, padded to whole chunks
-  const int cap = ((chunks + nranks - 1) / nranks) * kc;
-  const int acc = !a.acc ? NO_ACC : (long long)cap * (a.heads / a.kv_heads) * 4 <= SCORE_BYTES ? STORED : AGAIN;
+  // the most positions that one CTA may get, in whole chunks
+  auto cap = [&] { return (long long)((chunks + nranks - 1) / nranks) * kc; };
+  while (nranks < 8 && chunks > 4 * nranks &&
+         ((long long)a.batch * a.kv_heads * nranks < 3 * 148 || (a.acc && cap() * g * 4 > SCORE_BYTES)))
+    nranks *= 2;
+  const int acc = !a.acc ? NO_ACC : cap() * g * 4 <= SCORE_BYTES ? STORED : AGAIN;
   auto with = [&](auto t, auto d) {
     constexpr int T = decltype(t)::value, D = decltype(d)::value;
-    return acc == NO_ACC   ? launch<T, D, NO_ACC>(a, pre, nranks, cap, s)
-           : acc == STORED ? launch<T, D, STORED>(a, pre, nranks, cap, s)
-                           : launch<T, D, AGAIN>(a, pre, nranks, cap, s);
+    return acc == NO_ACC   ? launch<T, D, NO_ACC>(a, pre, nranks, (int)cap(), s)
+           : acc == STORED ? launch<T, D, STORED>(a, pre, nranks, (int)cap(), s)
+                           : launch<T, D, AGAIN>(a, pre, nranks, (int)cap(), s);
   };
   using I = std::integral_constant<int, 64>;
   using J = std::integral_constant<int, 128>;
