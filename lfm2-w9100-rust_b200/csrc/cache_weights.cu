@@ -11,12 +11,14 @@
 //   warp 1      TMEM and the MMAs, into two buffers of S^T
 //   warps 2-17  the sums; a key is shared by four threads, each for a quarter of the columns
 //   from 18 on  the rows' lse, and for fp32 queries the tiles: fp16 hi/lo pairs, two MMAs
-// Bound by the exponentials: 16 a cycle and SM, 2048 cycles for a tile of 128
-// keys and 256 rows. 8191 bf16 tokens of 32 heads and 128 values: 336 us, the special-function units
-// busy for 80% of it. A third of the exponentials through the fma units (range
-// reduction and a polynomial of degree 5) took the units' time down to 55% and left the total
-// (341 us): the issuing warp and the sums' start on each tile are what is left. Tiles of 128 rows
-// in four buffers: 350 us; eight warps for the sums: 434 us.
+// 16-bit queries are bound by the exponentials: 16 a cycle and SM, 2048 cycles for
+// a tile of 128 keys and 256 rows. 8191 bf16 tokens of 32 heads and 128 values: 345 us with the inputs in
+// L2, the special-function units busy for 80% of it, 370 us from memory. A third of
+// the exponentials through the fma units (range reduction and a polynomial of
+// degree 5) took the units' time down to 55% and left the total: the issuing warp
+// and the sums' start on each tile are what is left. Tiles of 128 rows in four buffers: 350 us;
+// eight warps for the sums: 434 us. fp32 queries are bound by making their pairs, once for each tile
+// of keys: 3840 tokens of 32 heads and 64 values 182 us with eight warps at it, 385 us with four.
 // A key is summed by one thread, in the order of the rows, tile by tile, and the
 // CTAs of a cluster that splits the rows are added up in their order: the
 // result is the same on every run.
@@ -38,7 +40,7 @@ template <int T, int D>
 struct Cfg {
   static constexpr bool PAIR = T == T_F32;
   static constexpr int N = PAIR && D == 128 ? 128 : 256;  // rows of a tile at most: two tiles have to fit
-  static constexpr int FEED = PAIR ? 4 : 2;  // warps that write lse, and fp32 queries
+  static constexpr int FEED = PAIR ? 8 : 2;               // warps that write lse, and fp32 queries
   static constexpr int THREADS = 32 * (2 + EPI + FEED);
   static constexpr int K_CHUNK = KEYS * 128, K_TILE = K_CHUNK * (D / 64);
   static constexpr int Q_CHUNK = N * 128, Q_TILE = Q_CHUNK * (D / 64), STAGE = (PAIR ? 2 : 1) * Q_TILE;
@@ -213,6 +215,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
   } else {
     // ---------------------------------------------------------- lse, fp32 queries
     const int ft = tid - 32 * (2 + EPI);
+    const int per_row = 65536 / a.g + 1;  // row / g = row * per_row >> 16 for rows of a tile
     constexpr int PER = (F::N + 32 * F::FEED - 1) / (32 * F::FEED), AHEAD = 4;
     float pre[AHEAD][PER];  // loaded AHEAD tiles before they are stored: under the tiles' traffic a load takes ~2700 cycles
     int off[PER];           // of a row's lse from that of its tile's first token
@@ -242,12 +245,13 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
       if constexpr (PAIR) {
         if (k >= F::RING && !(ok = mbar_wait(&empty[st], (k / F::RING - 1) & 1, nullptr))) return;
         uint8_t* dst = smem + F::K_TILE + st * F::STAGE;
-#pragma unroll 4
+#pragma unroll 2
         for (int i = ft; i < cols * (D / 8); i += 32 * F::FEED) {
           const int row = i / (D / 8), c = i % (D / 8);
           float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
           if (row < have) {
-            const float* q = a.q + (size_t)(t0 + row / a.g) * a.q_stride + (size_t)(kh * a.g + row % a.g) * D + 8 * c;
+            const int t = row * per_row >> 16;
+            const float* q = a.q + (size_t)(t0 + t) * a.q_stride + (size_t)(kh * a.g + row - t * a.g) * D + 8 * c;
             u = *(const float4*)q, w = *(const float4*)(q + 4);
           }
           const float f[8] = {u.x * a.scale2, u.y * a.scale2, u.z * a.scale2, u.w * a.scale2,
