@@ -22,11 +22,24 @@ lfm_status bad(const char* who, const char* what) {
 
 lfm_status done(const char* who, cudaError_t e) {
   if (e == cudaSuccess) return LFM_OK;
+  cudaGetLastError();  // reported here, not by the caller's next check
   char m[256];
   snprintf(m, sizeof m, "%s: CUDA: %s", who, cudaGetErrorString(e));
   lfm::ops_set_error(m);
   return LFM_ERR_CUDA;
 }
+
+// Whether the current device's kernels may read p: its own memory, or managed memory.
+bool here(const void* p) {
+  cudaPointerAttributes at;
+  int device = -1;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == device);
+}
+const char* const ELSEWHERE = "the arrays must be memory of the current device";
 
 bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
 
@@ -103,6 +116,11 @@ lfm_status decode_args(const char* who, const lfm_attn_shape* s, const void* q, 
   return LFM_OK;
 }
 
+bool decode_here(const Decode& a) {
+  return here(a.q) && here(a.k) && here(a.v) && here(a.lens) && here(a.out) && (!a.slots || here(a.slots)) &&
+         (!a.acc || here(a.acc));
+}
+
 struct Range {
   const char* p;
   size_t n;
@@ -120,6 +138,7 @@ lfm_status lfm_attention_window(const lfm_attn_shape* shape, const void* q, uint
   if (lfm_status st = prompt_args(who, shape, q, q_stride, k_cache, start, n, window, sinks, &a)) return st;
   if (const char* e = rows_error(shape, out, out_stride)) return bad(who, e);
   if (!v_cache || !aligned(v_cache)) return bad(who, "the caches must be 16-byte aligned device pointers");
+  if (!here(q) || !here(k_cache) || !here(v_cache) || !here(out) || (lse && !here(lse))) return bad(who, ELSEWHERE);
   a.v = v_cache, a.out = out, a.out_stride = out_stride, a.lse = lse;
   return done(who, lfm::cache::window(a, (cudaStream_t)stream));
 }
@@ -131,6 +150,7 @@ lfm_status lfm_attention_weights(const lfm_attn_shape* shape, const void* q, uin
   Prompt a;
   if (lfm_status st = prompt_args(who, shape, q, q_stride, k_cache, start, n, window, sinks, &a)) return st;
   if (!lse || !acc) return bad(who, "lse and acc must be device pointers");
+  if (!here(q) || !here(k_cache) || !here(lse) || !here(acc)) return bad(who, ELSEWHERE);
   a.lse = const_cast<float*>(lse), a.acc = acc;
   return done(who, lfm::cache::weights(a, (cudaStream_t)stream));
 }
@@ -147,6 +167,7 @@ lfm_status lfm_attention_decode(const lfm_attn_shape* shape, const void* q, uint
   a.window = window >= max_len ? 0 : (int)window;
   a.sinks = (int)(sinks < shape->ctx ? sinks : shape->ctx);
   a.acc = acc;
+  if (!decode_here(a)) return bad(who, ELSEWHERE);
   return done(who, lfm::cache::decode(a, (cudaStream_t)stream));
 }
 
@@ -174,6 +195,8 @@ lfm_status lfm_attention_shared(const lfm_attn_shape* shape, const void* q, uint
   a.pk = prefix_k, a.pv = prefix_v, a.prefix_ctx = (int)prefix_ctx, a.prefix_len = (int)prefix_len;
   if (!workspace || !aligned(workspace) || workspace_bytes < lfm::cache::shared_workspace(a))
     return bad(who, "workspace must be 16-byte aligned, of lfm_attention_shared_workspace bytes");
+  if (!decode_here(a) || !here(workspace) || (prefix_len && (!here(prefix_k) || !here(prefix_v))))
+    return bad(who, ELSEWHERE);
   a.work = workspace;
   return done(who, lfm::cache::shared(a, (cudaStream_t)stream));
 }
@@ -213,6 +236,12 @@ lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const
     for (int j = 0; j < i; j++)
       if (overlap(dst[i], dst[j])) return bad(who, "the destinations overlap one another");
   }
+  for (const Range& r : src)
+    if (r.p && !here(r.p)) return bad(who, ELSEWHERE);
+  for (const Range& r : dst)
+    if (r.p && !here(r.p)) return bad(who, ELSEWHERE);
+  for (const Range& r : in)
+    if (r.p && !here(r.p)) return bad(who, ELSEWHERE);
   Evict a = {};
   a.kv_heads = (int)shape->kv_heads, a.d = (int)shape->head_dim, a.ctx = (int)shape->ctx;
   a.k = k_src, a.v = v_src, a.acc = acc_src, a.pos = pos_src;

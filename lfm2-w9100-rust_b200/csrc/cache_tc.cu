@@ -68,6 +68,7 @@ struct Cfg {
 
 struct Rows {
   int heads, kv_heads, g, rows;  // rows of one KV head
+  int nranks;                    // CTAs that split a tile's positions
   float scale2;                  // scale * log2 e
   const void* q;
   size_t q_stride;
@@ -122,8 +123,9 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   __shared__ uint64_t q_full, k_full[F::RING], v_full[F::RING], s_full[F::RING], o_full[F::RING], p_full[2];
   __shared__ uint32_t tmem_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
-  const int r0 = (int)(gridDim.z - 1 - blockIdx.z) * ROWS;  // the longest rows first
+  // blockIdx.x counts ranks, then KV heads, then row tiles, the longest rows first
+  const int nranks = a.nranks, rank = blockIdx.x % nranks, kh = blockIdx.x / nranks % a.kv_heads;
+  const int r0 = (int)((gridDim.x - 1 - blockIdx.x) / nranks / a.kv_heads) * ROWS;
   const int nrows = min(ROWS, a.rows - r0);
   const Tiles tiles(a, r0, nrows);
   const int i0 = (int)((long long)tiles.n * rank / nranks), i1 = (int)((long long)tiles.n * (rank + 1) / nranks);
@@ -502,12 +504,12 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
 // CTAs that split one block's positions: as many as fill the SMs, each with a tile of its own at least.
 int split(int blocks, int tiles) {
   int n = 1;
-  while (n < 8 && 2 * n * blocks <= 2 * 148 && 2 * n <= tiles) n *= 2;
+  while (n < 8 && 2ll * n * blocks <= 2 * 148 && 2 * n <= tiles) n *= 2;
   return n;
 }
 
 template <int T, int D>
-cudaError_t launch(const Rows& a, const void* k, const void* v, int ctx, int tiles, cudaStream_t s) {
+cudaError_t launch(Rows a, const void* k, const void* v, int ctx, int tiles, cudaStream_t s) {
   using F = Cfg<T, D>;
   CUtensorMap mk, mv;
   cudaError_t e = map_cache(&mk, k, a.kv_heads, ctx, D, KT);
@@ -518,9 +520,9 @@ cudaError_t launch(const Rows& a, const void* k, const void* v, int ctx, int til
   static std::mutex mu;
   once_per_device(done, mu, [f] { cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
   const int blocks = (a.rows + ROWS - 1) / ROWS;
-  const int nranks = split(blocks * a.kv_heads, tiles);
+  const int nranks = a.nranks = split(blocks * a.kv_heads, tiles);
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(nranks, a.kv_heads, blocks);
+  c.gridDim = dim3((unsigned)nranks * a.kv_heads * blocks);
   c.blockDim = dim3(THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;

@@ -50,7 +50,7 @@ struct Cfg {
 };
 
 struct Args {
-  int heads, g, ctx;
+  int heads, kv_heads, g, ctx, nranks;
   float scale2;  // scale * log2 e
   const float* q;  // fp32 queries
   size_t q_stride;
@@ -73,8 +73,9 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
   __shared__ __align__(16) float s_lse[LSE_RING][F::N];  // -lse in log2 units
   __shared__ float s_sum[8][KEYS];                      // the quarters' sums, then those of the cluster's CTAs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y;
-  const int j0 = blockIdx.z * KEYS;  // the first keys, which most rows see, come first
+  // blockIdx.x counts ranks, then KV heads, then tiles: the first keys, which most rows see, come first
+  const int nranks = a.nranks, rank = blockIdx.x % nranks, kh = blockIdx.x / nranks % a.kv_heads;
+  const int j0 = blockIdx.x / nranks / a.kv_heads * KEYS;
   const int cols = a.tokens * a.g;
   // the tokens that see a key of this tile, in whole tiles, and this CTA's share of them
   const int first = max(0, j0 - a.start) / a.tokens;
@@ -309,7 +310,7 @@ template <int T, int D>
 cudaError_t launch(const Prompt& p, cudaStream_t s) {
   using F = Cfg<T, D>;
   Args a = {};
-  a.heads = p.heads, a.g = p.heads / p.kv_heads, a.ctx = p.ctx;
+  a.heads = p.heads, a.kv_heads = p.kv_heads, a.g = p.heads / p.kv_heads, a.ctx = p.ctx;
   a.scale2 = p.scale * LOG2E;
   a.q = (const float*)p.q, a.q_stride = p.q_stride;
   a.start = p.start, a.n = p.n, a.window = p.window, a.sinks = p.sinks;
@@ -331,9 +332,10 @@ cudaError_t launch(const Prompt& p, cudaStream_t s) {
   once_per_device(done, mu, [f] { cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
   const int tiles = (p.start + p.n + KEYS - 1) / KEYS, most = (p.n + a.tokens - 1) / a.tokens;
   int nranks = 1;
-  while (nranks < 8 && 2 * nranks * tiles * p.kv_heads <= 148 && 2 * nranks <= most) nranks *= 2;
+  while (nranks < 8 && 2ll * nranks * tiles * p.kv_heads <= 148 && 2 * nranks <= most) nranks *= 2;
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(nranks, p.kv_heads, tiles);
+  a.nranks = nranks;
+  c.gridDim = dim3((unsigned)nranks * p.kv_heads * tiles);
   c.blockDim = dim3(F::THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;

@@ -478,3 +478,137 @@ def test_serving_steps_together(cuda_lib):
         for x, y in zip((o1, o2, acc, pos, kd, lo), eager):
             assert torch.equal(x, y)
     assert status_of(cuda_lib) == 0
+
+
+def _shared_state(seed, batch=24, prefix=300, heads=8, kv=2, d=64, ctx=48):
+    import torch
+    rng = np.random.default_rng(seed)
+    sh = shape_of("bf16", heads, kv, d, ctx)
+    q = rows(rng, batch, heads * d, "bf16", heads * d).cuda()
+    k, v = (cache(rng, (batch, kv, ctx, d), "bf16").cuda() for _ in range(2))
+    pk, pv = (cache(rng, (kv, prefix, d), "bf16").cuda() for _ in range(2))
+    lens = torch.from_numpy(rng.integers(0, ctx + 1, batch).astype(np.int32)).cuda()
+    return sh, q, k, v, pk, pv, lens
+
+
+def _shared_call(lib, state, out, work, stream):
+    sh, q, k, v, pk, pv, lens = state
+    b, w = q.shape
+    check(lib.lfm_attention_shared(sh, ptr(q), w, ptr(pk), ptr(pv), pk.shape[1], pk.shape[1], ptr(k), ptr(v),
+                                   k.stride(0), b, None, ptr(lens), b, sh.ctx, ptr(out), w, ptr(work), work.numel(),
+                                   ctypes.c_void_p(stream.cuda_stream)), "shared")
+
+
+def test_shared_captured_replayed_and_on_two_streams(cuda_lib):
+    """The call's two kernels in a graph that is replayed after its inputs have changed, and two calls at once on two
+    streams with a workspace each."""
+    import torch
+    a, b = _shared_state(1), _shared_state(2)
+    need = cuda_lib.lfm_attention_shared_workspace(a[0], 24, 300)
+    work = [torch.zeros(need, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    want, main = [], torch.cuda.current_stream()
+    for s in (a, b):
+        out = torch.zeros_like(s[1])
+        _shared_call(cuda_lib, s, out, work[0], main)
+        want.append(out)
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.zeros_like(want[0]) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, o, w, t in zip((a, b), outs, work, side):
+            _shared_call(cuda_lib, s, o, w, t)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    out = torch.zeros_like(want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side[0]):
+        graph.capture_begin()
+        _shared_call(cuda_lib, a, out, work[0], side[0])
+        graph.capture_end()
+    for x, y in zip(a[1:], b[1:]):
+        x.copy_(y)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[1])
+    assert status_of(cuda_lib) == 0
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """No call needs one before it: the kernels' attributes and maps are set while the stream captures."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch, ctypes, conftest, lfm2_b200
+from test_gpu_cache_attn import _shared_state, _shared_call
+lib = lfm2_b200.lib()
+s = _shared_state(3)
+work = torch.zeros(lib.lfm_attention_shared_workspace(s[0], 24, 300), dtype=torch.uint8, device="cuda")
+out, again = torch.zeros_like(s[1]), torch.zeros_like(s[1])
+torch.cuda.synchronize()
+side, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+with torch.cuda.stream(side):
+    g.capture_begin()
+    _shared_call(lib, s, out, work, side)
+    g.capture_end()
+g.replay()
+torch.cuda.synchronize()
+_shared_call(lib, s, again, work, torch.cuda.current_stream())
+torch.cuda.synchronize()
+assert torch.equal(out, again) and bool((out != 0).any())
+print("same")
+""" % (here, os.path.join(os.path.dirname(here), "lfm2-w9100-rust_b200"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_offsets_past_32_bits(cuda_lib):
+    """A session whose cache starts 4.7e9 values into the array, its positions evicted in place there."""
+    import torch
+    kv, d, ctx, heads, slot = 8, 64, 1 << 17, 8, 70
+    stride = kv * ctx * d
+    k = torch.zeros((slot + 1) * stride, dtype=torch.float16, device="cuda")
+    v = torch.zeros((slot + 1) * stride, dtype=torch.float16, device="cuda")
+    rng = np.random.default_rng(4)
+    n = 200
+    q = rows(rng, 1, heads * d, "f16", heads * d)
+    kk, vv = cache(rng, (kv, n, d), "f16"), cache(rng, (kv, n, d), "f16")
+    at = slot * stride
+    kview, vview = k[at:].view(kv, ctx, d), v[at:].view(kv, ctx, d)
+    kview[:, :n], vview[:, :n] = kk.cuda(), vv.cuda()
+    sh = shape_of("f16", heads, kv, d, ctx)
+    sd, ld = torch.tensor([slot], dtype=torch.int32).cuda(), torch.tensor([n], dtype=torch.int32).cuda()
+    acc = torch.zeros(slot + 1, kv, ctx, device="cuda")
+    out = torch.zeros(1, heads * d, dtype=torch.float16, device="cuda")
+    qd, lo = q.cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    check(cuda_lib.lfm_attention_decode(sh, ptr(qd), heads * d, ptr(k), ptr(v), stride, slot + 1, ptr(sd), ptr(ld), 1,
+                                        ctx, 0, 0, ptr(acc), ptr(out), heads * d, None), "decode")
+    for h in range(heads):
+        o, _, w = attend(f64(q)[0, h * d:(h + 1) * d], f64(kk)[h], f64(vv)[h], np.ones(n, bool), d ** -0.5)
+        ds = score_error("f16", f64(q)[0, h * d:(h + 1) * d], f64(kk)[h], d ** -0.5)
+        tol = out_error("f16", ds, n, np.abs(f64(vv)[h]).max(), o)
+        assert (np.abs(out[0, h * d:(h + 1) * d].cpu().double().numpy() - o) <= tol).all()
+        assert np.abs(acc[slot, h, :n].cpu().double().numpy() - w).max() < 1e-5
+    assert acc[:slot].abs().max().item() == 0
+    check(cuda_lib.lfm_cache_evict(sh, ptr(k), ptr(v), ptr(acc), None, ptr(k), ptr(v), ptr(acc), None, stride, slot + 1,
+                                   ptr(sd), ptr(ld), ptr(lo), 1, n, 50, 0, 50, None), "evict")
+    assert torch.equal(kview[:, :50], kk[:, 150:].cuda()) and torch.equal(vview[:, :50], vv[:, 150:].cuda())
+    assert status_of(cuda_lib) == 0
+
+
+def test_memory_of_the_host_is_refused(cuda_lib):
+    import torch
+    x = torch.zeros(1 << 16)
+    y = torch.zeros(1 << 16, device="cuda")
+    sh = shape_of("f32", 8, 2, 64, 64)
+    assert cuda_lib.lfm_attention_window(sh, ptr(x), 512, ptr(y), ptr(y), 0, 4, 0, 0, ptr(y), 512, None, None) == 1
+    assert cuda_lib.lfm_attention_window(sh, ptr(y), 512, ptr(y), ptr(x), 0, 4, 0, 0, ptr(y), 512, None, None) == 1
+    assert cuda_lib.lfm_attention_weights(sh, ptr(y), 512, ptr(y), 0, 4, 0, 0, ptr(x), ptr(y), None) == 1
+    assert cuda_lib.lfm_attention_decode(sh, ptr(y), 512, ptr(y), ptr(y), 8192, 1, None, ptr(x), 1, 64, 0, 0, None,
+                                         ptr(y), 512, None) == 1
+    assert b"current device" in cuda_lib.lfm_ops_error()
