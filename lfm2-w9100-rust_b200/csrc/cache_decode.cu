@@ -40,11 +40,13 @@ using namespace dev;
 constexpr int STAGES = 2, HALF = 4096, STAGE = 2 * HALF;
 constexpr float LOG2E = 1.4426950408889634f;
 enum Acc { NO_ACC = 0, STORED = 1, AGAIN = 2 };
-// Three CTAs of 4 warps to an SM; where the scores are kept, one of 7 warps with what its ring leaves of shared memory
-// (24 sessions of up to 32768 positions, 6 heads of 128 values to a KV head: 288 us without weights).
+// Warps of a CTA. 4: three CTAs to an SM. 3: four, where that saves a second round (64 sessions of 1028 positions and 8
+// heads, 512 CTAs: 26 instead of 32 us; 256 sessions of 4 heads, 1024 CTAs: no gain). 7: where the scores are kept, one CTA
+// with what its ring leaves of shared memory (24 sessions of up to 32768 positions, 6 heads of 128 values to a KV head,
+// with weights: 356 us; reading K again 487 us; without weights 288 us).
 constexpr int warps_of(int acc) { return acc == STORED ? 7 : 4; }
-constexpr int ring_of(int acc) { return warps_of(acc) * STAGES * STAGE; }
-constexpr int SCORE_BYTES = 227 * 1024 - ring_of(STORED) - 6 * 1024;
+constexpr int ring_of(int warps) { return warps * STAGES * STAGE; }
+constexpr int SCORE_BYTES = 227 * 1024 - ring_of(warps_of(STORED)) - 6 * 1024;
 
 template <class C>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -68,11 +70,11 @@ struct Joint {
   const float2* ml;  // its (m in log2 units, l) [kv head][row]
 };
 
-template <int T, int D, int ACC>
-__global__ void __launch_bounds__(warps_of(ACC) * 32) k_decode(Decode a, Joint pre, int cap) {
+template <int T, int D, int ACC, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int cap) {
   using Q = typename Types<T>::Q;
   using C = typename Types<T>::C;
-  constexpr int WARPS = warps_of(ACC), RING = ring_of(ACC);
+  constexpr int RING = ring_of(WARPS);
   constexpr int KC = HALF / (2 * D);  // positions of a chunk
   constexpr int NU = D / 64, TILES = KC / 8;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -388,18 +390,18 @@ __global__ void __launch_bounds__(warps_of(ACC) * 32) k_decode(Decode a, Joint p
   }
 }
 
-template <int T, int D, int ACC>
+template <int T, int D, int ACC, int WARPS = warps_of(ACC)>
 cudaError_t launch(const Decode& a, const Joint& pre, int nranks, int cap, cudaStream_t s) {
-  const int smem = ring_of(ACC) + (ACC == STORED ? a.heads / a.kv_heads * cap * 4 : 0);
-  auto* f = k_decode<T, D, ACC>;
+  const int smem = ring_of(WARPS) + (ACC == STORED ? a.heads / a.kv_heads * cap * 4 : 0);
+  auto* f = k_decode<T, D, ACC, WARPS>;
   static unsigned long long done = 0;
   static std::mutex mu;
   once_per_device(done, mu, [f] {
-    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_of(ACC) + (ACC == STORED ? SCORE_BYTES : 0));
+    cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_of(WARPS) + (ACC == STORED ? SCORE_BYTES : 0));
   });
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(nranks, a.kv_heads, a.batch);
-  c.blockDim = dim3(warps_of(ACC) * 32);
+  c.blockDim = dim3(WARPS * 32);
   c.dynamicSmemBytes = smem;
   c.stream = s;
   cudaLaunchAttribute at[2];
@@ -428,6 +430,8 @@ cudaError_t run(const Decode& a, const Joint& pre, cudaStream_t s) {
   const int acc = !a.acc ? NO_ACC : cap() * g * 4 <= SCORE_BYTES ? STORED : AGAIN;
   auto with = [&](auto t, auto d) {
     constexpr int T = decltype(t)::value, D = decltype(d)::value;
+    const long long ctas = (long long)a.batch * a.kv_heads * nranks;
+    if (acc == NO_ACC && ctas > 3 * 148 && ctas <= 4 * 148) return launch<T, D, NO_ACC, 3>(a, pre, nranks, (int)cap(), s);
     return acc == NO_ACC   ? launch<T, D, NO_ACC>(a, pre, nranks, (int)cap(), s)
            : acc == STORED ? launch<T, D, STORED>(a, pre, nranks, (int)cap(), s)
                            : launch<T, D, AGAIN>(a, pre, nranks, (int)cap(), s);

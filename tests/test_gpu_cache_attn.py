@@ -170,6 +170,8 @@ DECODE = [  # kind, heads, kv, d, ctx, lens, window, sinks, acc, pad
     ("bf16", 7, 7, 64, 90, [90, 89, 5], 50, 60, False, 8),
     ("bf16", 8, 1, 128, 9000, [9000], 0, 0, True, 0),
     ("f16", 8, 1, 64, 60000, [60000, 0, 53], 0, 0, True, 0),
+    ("f32", 16, 8, 64, 70, [i * 70 // 63 for i in range(64)], 40, 3, False, 0),  # more CTAs than fit three to an SM
+    ("bf16", 8, 4, 128, 70, [70 - i * 70 // 129 for i in range(130)], 0, 0, False, 8),
 ]
 
 
