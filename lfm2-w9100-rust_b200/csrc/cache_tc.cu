@@ -236,12 +236,17 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     const int R = r0 + min(row, nrows - 1), tok = R / a.g, head = kh * a.g + R % a.g;
     const bool live = row < nrows;
     {
-      const Q* q = (const Q*)a.q + (size_t)tok * a.q_stride + (size_t)head * D;
+      // Rows behind the last are copies of it. fp32: a row's 8-value pieces go to neighbouring threads (3840 tokens 98.8
+      // -> 96.9 us). 16 bits: a thread loads its own row; the other way took 238 instead of 232 us for 8192 tokens of 128
+      // values, and 114 instead of 115 us for 256 sessions behind a prefix.
 #pragma unroll
-      for (int c = 0; c < D / 8; c++) {
+      for (int k = 0; k < D / 8; k++) {
+        const int i = tid - 64 + 128 * k, qr = PAIR ? i / (D / 8) : row, c = PAIR ? i % (D / 8) : k;
+        const int QR = r0 + min(qr, nrows - 1), qt = QR / a.g;
+        const Q* q = (const Q*)a.q + (size_t)qt * a.q_stride + (size_t)(kh * a.g + QR - qt * a.g) * D + 8 * c;
         uint8_t* chunk = smem + (c >> 3) * F::Q_CHUNK;
         if constexpr (PAIR) {
-          const float4 u = *(const float4*)(q + 8 * c), v = *(const float4*)(q + 8 * c + 4);
+          const float4 u = *(const float4*)q, v = *(const float4*)(q + 4);
           const float f[8] = {u.x * a.scale2, u.y * a.scale2, u.z * a.scale2, u.w * a.scale2,
                               v.x * a.scale2, v.y * a.scale2, v.z * a.scale2, v.w * a.scale2};
           uint32_t h[4], l[4];
@@ -250,10 +255,10 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
             h[e] = pack(__half(), f[2 * e], f[2 * e + 1]);
             l[e] = rest(h[e], f[2 * e], f[2 * e + 1]);
           }
-          st_piece(chunk, row, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
-          st_piece(chunk + F::Q_TILE, row, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
+          st_piece(chunk, qr, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
+          st_piece(chunk + F::Q_TILE, qr, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
         } else {
-          st_piece(chunk, row, c & 7, *(const uint4*)(q + 8 * c));
+          st_piece(chunk, qr, c & 7, *(const uint4*)q);
         }
       }
       fence_async_smem();
