@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
   const int rank = blockIdx.x, nranks = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
   const int g = a.heads / a.kv_heads;
 
+  // what is before this kernel, or, behind the prefix's kernel, which has waited for that, later: that kernel's part
+  if (!pre.o) pdl_wait();
   int slot, len;
   const bool good = session(a.slots, a.lens, b, a.n_slots, a.max_len, &slot, &len);
   if (!good) slot = len = 0;
@@ -407,10 +409,10 @@ cudaError_t launch(const Decode& a, const Joint& pre, int nranks, int cap, cudaS
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = nranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits for what is before it (pdl_wait)
   at[1].val.programmaticStreamSerializationAllowed = 1;
   c.attrs = at;
-  c.numAttrs = pre.o ? 2 : 1;
+  c.numAttrs = 2;
   return cudaLaunchKernelEx(&c, f, a, pre, cap);
 }
 

@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_evict(Evict a, bool in_place) {
   __shared__ int s_warp[WARPS], s_found[2], s_dup;
   const int rank = blockIdx.x, nranks = gridDim.x, h = blockIdx.y, b = blockIdx.z;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();  // up to here the kernel may run beside the one before it
   int slot, len;
   if (!session(a.slots, a.lens, b, a.n_slots, a.max_len, &slot, &len)) return;
   if (a.slots) {
@@ -221,11 +222,13 @@ cudaError_t evict(const Evict& a, cudaStream_t s) {
   c.gridDim = dim3(nranks, a.kv_heads, a.batch);
   c.blockDim = dim3(THREADS);
   c.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = nranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits for what is before it (pdl_wait)
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   c.attrs = at;
-  c.numAttrs = 1;
+  c.numAttrs = 2;
   return a.d == 64 ? cudaLaunchKernelEx(&c, k_evict<64>, a, a.k == a.k_out)
                    : cudaLaunchKernelEx(&c, k_evict<128>, a, a.k == a.k_out);
 }

@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
+  pdl_wait();  // up to here the kernel may run beside the one before it
   if (nranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
 
   if (warp < 2) {
@@ -531,11 +532,13 @@ cudaError_t launch(Rows a, const void* k, const void* v, int ctx, int tiles, cud
   c.blockDim = dim3(THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = nranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits for what is before it (pdl_wait)
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   c.attrs = at;
-  c.numAttrs = 1;
+  c.numAttrs = 2;
   return cudaLaunchKernelEx(&c, f, mk, mv, a);
 }
 

@@ -105,6 +105,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
+  pdl_wait();  // up to here the kernel may run beside the one before it
   if (nranks > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   bool ok = true;
   float sum = 0.f;
@@ -339,11 +340,13 @@ cudaError_t launch(const Prompt& p, cudaStream_t s) {
   c.blockDim = dim3(F::THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = nranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits for what is before it (pdl_wait)
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   c.attrs = at;
-  c.numAttrs = 1;
+  c.numAttrs = 2;
   return cudaLaunchKernelEx(&c, f, mk, mq, a);
 }
 }  // namespace
