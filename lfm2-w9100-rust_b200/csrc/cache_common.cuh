@@ -14,7 +14,8 @@ namespace cache {
 static __device__ unsigned g_status;
 __device__ __forceinline__ void report(unsigned bits) { atomicOr(&g_status, bits); }
 
-inline cudaError_t take_status(unsigned* bits, cudaStream_t s) {
+// (static, like the variable: each file has its own)
+static cudaError_t take_status(unsigned* bits, cudaStream_t s) {
   unsigned *at = nullptr, got = 0;
   cudaError_t e = cudaGetSymbolAddress((void**)&at, g_status);
   if (e == cudaSuccess) e = cudaMemcpyAsync(&got, at, sizeof got, cudaMemcpyDeviceToHost, s);
@@ -43,9 +44,6 @@ struct Types<T_BF16> {
   using C = __nv_bfloat16;
 };
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
 __device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
@@ -57,19 +55,6 @@ __device__ __forceinline__ uint32_t peer(const void* p, uint32_t rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(dev::smem_u32(p)), "r"(rank));
   return r;
-}
-__device__ __forceinline__ float ld_peer(uint32_t at) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 ld_peer4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at)
-               : "memory");
-  return v;
 }
 
 // 2^x by the hardware's instruction, within 2^-22 of it; results under 2^-126 are 0.

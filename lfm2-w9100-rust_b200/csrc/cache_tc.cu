@@ -54,7 +54,7 @@ struct Cfg {
   static constexpr int Q_CHUNK = ROWS * 128, KV_CHUNK = KT * 128;  // rows x 64 16-bit values, swizzled
   static constexpr int Q_TILE = Q_CHUNK * (D / 64), TILE = KV_CHUNK * (D / 64);
   static constexpr int Q_BYTES = (PAIR ? 2 : 1) * Q_TILE;
-  static constexpr int STATIC = 3072, RESERVED = 1024;  // of the kernel's static arrays, of the system
+  static constexpr int STATIC = 2048, RESERVED = 1024;  // of the kernel's static arrays, of the system
   // two CTAs to an SM, except for fp32 queries of 128 values, whose pairs leave no room for the second one's ring
   static constexpr int CTAS = PAIR && D == 128 ? 1 : 2;
   static constexpr int RING = std::min(4, (228 * 1024 / CTAS - STATIC - RESERVED - Q_BYTES) / (2 * TILE));  // K and V tiles each

@@ -34,11 +34,6 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
       " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ bool elect() {
-  uint32_t one;
-  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(one));
-  return one != 0;
-}
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
   asm volatile(
