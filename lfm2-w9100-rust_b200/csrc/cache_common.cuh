@@ -44,6 +44,17 @@ struct Types<T_BF16> {
   using C = __nv_bfloat16;
 };
 
+// Weights that enter a product in fp16 are taken relative to a row's reference of
+// log2 m = its maximum - SHIFT, not to the maximum: the type's exponents above 1
+// would lie idle, and below 2^-14 (low halves of a pair: 2^-3) its steps stop
+// shrinking. With 2^15 the steps of a pair are relative down to 2^-18 of the
+// largest weight and 2^-40 of it below; with 0 a key that takes all the weight
+// over a small V row left 4e-5 (6 nats above the others) to 8e-2 (14) of error
+// in fp32 outputs. Sums and outputs carry the same factor, which cancels; bf16
+// has fp32's exponents.
+template <int T>
+constexpr float SHIFT = T == T_BF16 ? 0.f : 15.f;
+
 __device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
 __device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }

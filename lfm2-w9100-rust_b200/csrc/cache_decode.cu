@@ -19,7 +19,11 @@
 //       lane reads the same 16 bytes of 4 positions and pairs them by byte
 //       permutes; output column n of tile e is head_dim index 8 n + e.
 // Statistics and outputs stay in fp32; exponentials are of powers of two (the
-// queries or the scores carry scale * log2 e). The warps join through shared
+// queries or the scores carry scale * log2 e), relative to the maximum less
+// SHIFT (cache_common.cuh). 16-bit queries: the weights are rounded to the
+// caches' type, half a step each (fp16 2^-11, bf16 2^-8), as the caller's V and
+// output are; pairs would double the products. The sums l are of the weights as
+// they were. The warps join through shared
 // memory, the CTAs through the cluster's: each sends its part of the columns to
 // the CTA that finishes them, so a call is one launch without workspace. Accumulated weights need
 // the joined statistics: a CTA keeps its scores in shared memory until the
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
 #pragma unroll
     for (int kt = 0; kt < TILES; kt++) mx = fmaxf(mx, fmaxf(s[kt][0], s[kt][1]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) - SHIFT<T>;
     if constexpr (ACC == STORED) {
       if (r < g) {
         float* dst = scores + r * cap + (i0 - c0 * KC) + 2 * t;
@@ -356,13 +360,14 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
       if constexpr (ACC == STORED) {
         for (int i = tid; i < count; i += WARPS * 32) {
           float sum = 0.f;
-          for (int h = 0; h < g; h++) sum = fmaf(exp2_fast(scores[h * cap + i] - f_m[h]), f_inv[h], sum);
+          for (int h = 0; h < g; h++)
+            sum = fmaf(exp2_fast(scores[h * cap + i] - (f_m[h] + SHIFT<T>)), f_inv[h] * exp2f(SHIFT<T>), sum);
           const int j = first + i;
           atomicAdd(acc + (j < hi ? j : lo + j - hi), sum);
         }
       } else {
         // K once more: the ring's barriers go on from the phases that the first walk left
-        const float M = f_m[min(r, g - 1)], inv = r < g ? f_inv[r] : 0.f;
+        const float M = f_m[min(r, g - 1)] + SHIFT<T>, inv = r < g ? f_inv[r] * exp2f(SHIFT<T>) : 0.f;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring was written by this warp's stores
         __syncthreads();
         if (lane == 0 && ok)

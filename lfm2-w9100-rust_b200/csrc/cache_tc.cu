@@ -18,8 +18,13 @@
 // of which either unit was busy for half: 282 us for 8192 tokens, window 1500.)
 //
 // 16-bit queries: O stays in tensor memory, and a row's maximum is raised, and O
-// rescaled, only when it grows by more than 2^8, which keeps every weight inside
-// fp16's range and every rounding relative. fp32 queries: q and P are fp16 hi/lo
+// rescaled, only when it grows by more than 2^8. Weights are relative to the
+// maximum less TOP, which keeps them inside fp16's range up to that growth and
+// their roundings relative (fp16: down to 2^-21 of the largest). They are
+// rounded to the caches' type, half a step each (fp16 2^-11, bf16 2^-8), as the
+// caller's V and output are: pairs would double the second product. The sums l
+// are of the weights as they were. Together with the output's own rounding that
+// is 2.2e-3 of error in bf16 (1.6e-3 with fp32 weights). fp32 queries: q and P are fp16 hi/lo
 // pairs, two MMAs each, the low parts first; the tensor core cuts its sums off
 // instead of rounding them, a loss that grows with their number (2.2e-6 over
 // 1024 positions), so O of each tile starts from zero and is added to the
@@ -46,6 +51,9 @@ using namespace tc;
 constexpr int THREADS = 192, KT = 64, ROWS = 128;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float GROWTH = 8.f;  // log2 of what a row may grow before its maximum is raised
+// log2 of the largest weight when the maximum has just been raised: fp16 keeps room for GROWTH
+template <int T>
+constexpr float TOP = T == T_F16 ? SHIFT<T> - GROWTH : SHIFT<T>;
 constexpr uint32_t COLS = 256, COL_O = 2 * KT;  // tensor memory: two buffers of S, then those of O
 
 template <int T, int D>
@@ -81,6 +89,12 @@ struct Rows {
   float* part;     // prefix: O [kv head][row][D], not divided
   float2* part_ml; // prefix: (m in log2 units, l)
 };
+
+// ln of 2^m l; the sum without its factor, so that the logarithm is of a number near 1 or above.
+template <int T>
+__device__ __forceinline__ float log_sum(float m, float l) {
+  return ((m + TOP<T>) + log2f(l * exp2f(-TOP<T>))) * LN2;
+}
 
 // The position tiles of a block of rows: the sinks in front of the window, then
 // the positions from the first row's window to the last row. A tile has `width`
@@ -336,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
             mx = fmaxf(mx, most(c));
           }
       }
-      mx *= sc;
+      mx = mx * sc - TOP<T>;
       float alpha = 1.f;
       if (PAIR || __any_sync(0xffffffffu, mx > m + GROWTH)) {
         const float mn = fmaxf(m, mx);
@@ -423,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           if (a.prefix)
             a.part_ml[at] = make_float2(m, l);
           else if (a.lse)
-            a.lse[(size_t)tok * a.heads + head] = (m + log2f(l)) * LN2;
+            a.lse[(size_t)tok * a.heads + head] = log_sum<T>(m, l);
         }
       }
     } else {
@@ -486,7 +500,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           const float inv = 1.f / L;
           store4((Q*)a.out + (size_t)tok2 * a.out_stride + (size_t)head2 * D + c,
                  make_float4(f.x * inv, f.y * inv, f.z * inv, f.w * inv));
-          if (c == 0 && a.lse) a.lse[(size_t)tok2 * a.heads + head2] = (M + log2f(L)) * LN2;
+          if (c == 0 && a.lse) a.lse[(size_t)tok2 * a.heads + head2] = log_sum<T>(M, L);
         }
       }
     }

@@ -1,0 +1,88 @@
+"""Precision of the session-cache attention calls against 64-bit values, in
+norm and on the inputs where a number format shows (limits: cache_attn_norm)."""
+
+import numpy as np
+import pytest
+
+from cache_attn_norm import SHIFT, dominated, fp16_floor, limit, norm_error, plain32, score_cut
+from cache_attn_ref import attend, ptr, torch_types
+from test_gpu_cache_attn import check, f64, shape_of, status_of
+
+pytestmark = pytest.mark.gpu
+
+
+def on_gpu(x, kind, cache):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(x)).to(torch_types(kind)[1 if cache else 0]).cuda()
+
+
+def decode(lib, kind, heads, q, k, v, lens, acc=None):
+    """q [batch][heads * d], k and v [batch][kv][ctx][d]."""
+    import torch
+    batch, kv, ctx, d = k.shape
+    out = torch.full_like(q, float("nan"))
+    ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    check(lib.lfm_attention_decode(shape_of(kind, heads, kv, d, ctx), ptr(q), heads * d, ptr(k), ptr(v), kv * ctx * d,
+                                   batch, None, ptr(ld), batch, max(lens), 0, 0, ptr(acc), ptr(out), heads * d, None),
+          "decode")
+    return out
+
+
+def window(lib, kind, heads, q, k, v, start, lse=None):
+    """q [n][heads * d], k and v [kv][ctx][d]."""
+    import torch
+    kv, ctx, d = k.shape
+    out = torch.full_like(q, float("nan"))
+    check(lib.lfm_attention_window(shape_of(kind, heads, kv, d, ctx), ptr(q), heads * d, ptr(k), ptr(v), start, len(q),
+                                   0, 0, ptr(out), heads * d, ptr(lse), None), "window")
+    return out
+
+
+def shared(lib, kind, heads, q, pk, pv, k, v, lens):
+    """q [batch][heads * d], pk and pv [kv][prefix][d], k and v [batch][kv][ctx][d]."""
+    import torch
+    batch, kv, ctx, d = k.shape
+    prefix = pk.shape[1]
+    sh = shape_of(kind, heads, kv, d, ctx)
+    out = torch.full_like(q, float("nan"))
+    ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    need = lib.lfm_attention_shared_workspace(sh, batch, prefix)
+    work = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    check(lib.lfm_attention_shared(sh, ptr(q), heads * d, ptr(pk), ptr(pv), prefix, prefix, ptr(k), ptr(v), kv * ctx * d,
+                                   batch, None, ptr(ld), batch, max(max(lens), 1), ptr(out), heads * d, ptr(work), need,
+                                   None), "shared")
+    return out
+
+
+def row_errors(kind, q, k, v, got, growth=0.0):
+    """The error in norm and its limit for rows got [heads][d] over k, v [kv][n][d]; `growth` is the power of two that
+    the kernel leaves free above the largest weight (fp16 queries of many rows: 2^8)."""
+    heads, d = q.shape
+    g, every = heads // len(k), np.ones(k.shape[1], bool)
+    rows = [attend(q[h], k[h // g], v[h // g], every, d ** -0.5) for h in range(heads)]
+    want = np.stack([r[0] for r in rows])
+    floor = np.linalg.norm([fp16_floor(r[2], v[h // g], SHIFT[kind] - growth) for h, r in enumerate(rows)])
+    floor = 0.0 if kind == "bf16" else floor / np.linalg.norm(want)
+    floor += max(score_cut(d, k[h // g] @ q[h] * d ** -0.5) for h in range(heads))
+    plain = np.stack([plain32(q[h], k[h // g], v[h // g], d ** -0.5) for h in range(heads)])
+    return norm_error(got, want), limit(kind, norm_error(plain, want), floor)
+
+
+@pytest.mark.parametrize("kind,d,nats", [(kind, d, nats) for kind in ("f32", "f16", "bf16") for d in (64, 128)
+                                         for nats in (6, 10) + ((14,) if kind != "f16" else ())])
+def test_a_key_that_takes_the_weight_over_a_zero_value(cuda_lib, kind, d, nats):
+    """A sink's place: one key far above the others, its value row 0. The error is relative to what is left."""
+    heads, kv, n, at = 8, 2, 3000, 3
+    q, k, v = dominated(np.random.default_rng(d + nats), kind, heads, kv, n, d, nats, at)
+    qd, kd, vd = on_gpu(q.reshape(1, -1), kind, False), on_gpu(k, kind, True), on_gpu(v, kind, True)
+    empty = kd[None, :, :1].contiguous(), vd[None, :, :1].contiguous()
+    outs = {"decode": decode(cuda_lib, kind, heads, qd, kd[None], vd[None], [n]),
+            "window": window(cuda_lib, kind, heads, qd, kd, vd, n - 1),
+            "shared": shared(cuda_lib, kind, heads, qd, kd, vd, *empty, [0]),
+            "joined": shared(cuda_lib, kind, heads, qd, kd[:, :1000].contiguous(), vd[:, :1000].contiguous(),
+                             kd[None, :, 1000:].contiguous(), vd[None, :, 1000:].contiguous(), [n - 1000])}
+    assert status_of(cuda_lib) == 0
+    for name, out in outs.items():
+        error, most = row_errors(kind, q, k, v, f64(out.cpu()).reshape(heads, d),
+                                 8.0 if kind == "f16" and name != "decode" else 0.0)
+        assert error <= most, (name, error, most)
