@@ -12,6 +12,9 @@
 // query heads. For fp32 queries the row r + 8 holds what the fp16 row r leaves
 // off (hi/lo pairs of q and of the weights), so one instruction does both halves
 // and the sum of the two accumulator rows, which one thread holds, has ~22 bits.
+// A chunk's output is added to the running one in fp32: accumulated in the matrix
+// unit, which cuts its sums off, outputs came out smaller by 1.6e-5 of themselves
+// over 2048 positions of a warp and by 6.6e-5 over 8192.
 //   S = Q K^T: a lane reads 16 bytes of one key's row; the order of the
 //       head_dim terms that this gives the instruction's k index is the same
 //       for q, whose fragments are laid out to match. No transposed load.
@@ -49,6 +52,7 @@ enum Acc { NO_ACC = 0, STORED = 1, AGAIN = 2 };
 // with what its ring leaves of shared memory (24 sessions of up to 32768 positions, 6 heads of 128 values to a KV head,
 // with weights: 356 us; reading K again 487 us; without weights 288 us).
 constexpr int warps_of(int acc) { return acc == STORED ? 7 : 4; }
+constexpr int ctas_of(int warps) { return warps == 3 ? 4 : warps == 4 ? 3 : 1; }  // to an SM, by their rings
 constexpr int ring_of(int warps) { return warps * STAGES * STAGE; }
 constexpr int SCORE_BYTES = 227 * 1024 - ring_of(warps_of(STORED)) - 6 * 1024;
 
@@ -75,7 +79,7 @@ struct Joint {
 };
 
 template <int T, int D, int ACC, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int cap) {
+__global__ void __launch_bounds__(WARPS * 32, ctas_of(WARPS)) k_decode(Decode a, Joint pre, int cap) {
   using Q = typename Types<T>::Q;
   using C = typename Types<T>::C;
   constexpr int RING = ring_of(WARPS);
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
     }
   };
 
-  float m = -INFINITY, l = 0.f, o[NU][8][4] = {};
+  float m = -INFINITY, l = 0.f, o[NU][8][2] = {};  // o: head r, column 64 u + 8 (2 t + x) + e
   bool ok = true;
   for (int i = 0; i < mine && ok; i++) {
     const int st = i % STAGES, i0 = (c0 + w + i * WARPS) * KC;
@@ -203,16 +207,12 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
         for (int kt = 0; kt < TILES; kt++) *(float2*)(dst + 8 * kt) = make_float2(s[kt][0], s[kt][1]);
       }
     }
+    float alpha = 1.f;
     if (__any_sync(0xffffffffu, mx > m)) {
-      const float mn = fmaxf(m, mx), alpha = part_weight(m, mn);
+      const float mn = fmaxf(m, mx);
+      alpha = part_weight(m, mn);
       m = mn;
       l *= alpha;
-#pragma unroll
-      for (int u = 0; u < NU; u++)
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-#pragma unroll
-          for (int x = 0; x < 4; x++) o[u][e][x] *= alpha;
     }
     uint32_t p[TILES][2];  // [tile][hi, lo]
 #pragma unroll
@@ -235,11 +235,13 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
         p[kt][1] = 0u;
       }
     }
+    // a chunk's output starts from zero and is added in fp32: the matrix unit cuts its sums off
 #pragma unroll
-    for (int kk = 0; kk < TILES / 2; kk++) {
-      const uint32_t pa[4] = {p[2 * kk][0], p[2 * kk][1], p[2 * kk + 1][0], p[2 * kk + 1][1]};
+    for (int u = 0; u < NU; u++) {
+      float c[8][4] = {};
 #pragma unroll
-      for (int u = 0; u < NU; u++) {
+      for (int kk = 0; kk < TILES / 2; kk++) {
+        const uint32_t pa[4] = {p[2 * kk][0], p[2 * kk][1], p[2 * kk + 1][0], p[2 * kk + 1][1]};
         uint32_t v[4][4];
 #pragma unroll
         for (int x = 0; x < 4; x++) {
@@ -249,10 +251,14 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const uint32_t sel = e & 1 ? 0x7632u : 0x5410u;
-          mma16816<C>(o[u][e], pa, __byte_perm(v[0][e >> 1], v[1][e >> 1], sel),
+          mma16816<C>(c[e], pa, __byte_perm(v[0][e >> 1], v[1][e >> 1], sel),
                       __byte_perm(v[2][e >> 1], v[3][e >> 1], sel));
         }
       }
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) o[u][e][x] = fmaf(o[u][e][x], alpha, PAIR ? c[e][x] + c[e][x + 2] : c[e][x]);
     }
     __syncwarp();
     if (lane == 0 && i + STAGES < mine) fetch(i + STAGES, st, true);
@@ -274,11 +280,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_decode(Decode a, Joint pre, int 
       float* dst = wo + r * D + 64 * u + 8 * (2 * t + x);
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
-        float4 f;
-        f.x = PAIR ? o[u][e][x] + o[u][e][x + 2] : o[u][e][x];
-        f.y = PAIR ? o[u][e + 1][x] + o[u][e + 1][x + 2] : o[u][e + 1][x];
-        f.z = PAIR ? o[u][e + 2][x] + o[u][e + 2][x + 2] : o[u][e + 2][x];
-        f.w = PAIR ? o[u][e + 3][x] + o[u][e + 3][x + 2] : o[u][e + 3][x];
+        const float4 f = make_float4(o[u][e][x], o[u][e + 1][x], o[u][e + 2][x], o[u][e + 3][x]);
         *(float4*)(dst + e) = f;
       }
     }

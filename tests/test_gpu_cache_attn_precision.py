@@ -86,3 +86,43 @@ def test_a_key_that_takes_the_weight_over_a_zero_value(cuda_lib, kind, d, nats):
         error, most = row_errors(kind, q, k, v, f64(out.cpu()).reshape(heads, d),
                                  8.0 if kind == "f16" and name != "decode" else 0.0)
         assert error <= most, (name, error, most)
+
+
+def long_rows(seed, kind, heads, kv, n, d, batch):
+    """Queries, and keys and values of n positions that every session shares, the values positive: an error that grows
+    with the number of positions adds up instead of averaging out."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    qt, ct = torch_types(kind)
+    q = torch.randn(batch, heads * d, generator=g, device="cuda").to(qt)
+    k = torch.randn(kv, n, d, generator=g, device="cuda").to(ct)
+    v = (torch.rand(kv, n, d, generator=g, device="cuda") + 0.5).to(ct)
+    return q, k, v
+
+
+def long_reference(q, k, v, heads):
+    """64-bit outputs [batch][heads][d]."""
+    import torch
+    kv, _, d = k.shape
+    x = q.double().view(-1, kv, heads // kv, d) * d ** -0.5
+    out = torch.stack([torch.softmax(x[:, h] @ k[h].double().T, -1) @ v[h].double() for h in range(kv)], 1)
+    return out.reshape(-1, heads, d)
+
+
+# What a long sum may lose in the mean of all outputs. fp32 queries: a tile or chunk of up to eight sums cut off by less
+# than 2^-23 each. fp16: the same up to a fold, 256 sums on the way up to the value, half a step of 2^-23 lost in the mean
+# of each, and six standard deviations of the mean of `count` roundings to fp16 (uniform in half a step of 2^-11).
+def most_bias(kind, count):
+    return 8 * 2.0 ** -23 if kind == "f32" else 256 * 2.0 ** -25 + 6 * 2.0 ** -11 / np.sqrt(3 * count)
+
+
+@pytest.mark.parametrize("kind,heads,kv,n,d,batch", [("f32", 8, 2, 16385, 64, 80), ("f32", 8, 1, 200001, 128, 1),
+                                                     ("f32", 4, 1, 1 << 20, 64, 1), ("f16", 8, 1, 1 << 20, 64, 1)])
+def test_long_sums_of_one_token(cuda_lib, kind, heads, kv, n, d, batch):
+    q, k, v = long_rows(n, kind, heads, kv, n, d, batch)
+    every = [x[None].expand(batch, kv, n, d).contiguous() for x in (k, v)]
+    out = decode(cuda_lib, kind, heads, q, *every, [n] * batch)
+    want = long_reference(q, k, v, heads)
+    bias = ((out.double().view_as(want) - want) / want).mean().item()
+    assert status_of(cuda_lib) == 0
+    assert abs(bias) <= most_bias(kind, want.numel()), bias
