@@ -18,7 +18,8 @@
 // of which either unit was busy for half: 282 us for 8192 tokens, window 1500.)
 //
 // 16-bit queries: O stays in tensor memory, and a row's maximum is raised, and O
-// rescaled, only when it grows by more than 2^8. Weights are relative to the
+// rescaled, only when it grows by more than 2^8; over long rows it is moved every FOLD tiles into
+// a running output. Weights are relative to the
 // maximum less TOP, which keeps them inside fp16's range up to that growth and
 // their roundings relative (fp16: down to 2^-21 of the largest). They are
 // rounded to the caches' type, half a step each (fp16 2^-11, bf16 2^-8), as the
@@ -96,6 +97,10 @@ __device__ __forceinline__ float log_sum(float m, float l) {
   return ((m + TOP<T>) + log2f(l * exp2f(-TOP<T>))) * LN2;
 }
 
+// Tiles whose output 16-bit queries add up in tensor memory, which cuts the sums off: 256 sums lose at most 3e-5, 1/16
+// of fp16's half step. Without the fold a row of 2^20 positions came out smaller by 8e-4.
+constexpr int FOLD = 64;
+
 // The position tiles of a block of rows: the sinks in front of the window, then
 // the positions from the first row's window to the last row. A tile has `width`
 // columns (32 or 64) of which the first `valid` exist. Every row sees all of the
@@ -121,13 +126,14 @@ struct Tiles {
   __device__ __forceinline__ int width(int i) const { return all(i) || valid(i) > 32 ? 64 : 32; }
 };
 
-template <int T, int D>
+template <int T, int D, bool LONG>
 __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     k_rows(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Rows a) {
   using F = Cfg<T, D>;
   using Q = typename Types<T>::Q;
   using C = typename Types<T>::C;
   constexpr bool PAIR = F::PAIR;
+  static_assert(!(PAIR && LONG), "fp32 queries fold every tile");
   constexpr uint32_t BF = std::is_same<C, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* ring = smem + F::Q_BYTES;  // K and V of ring place 0, of place 1, ...
@@ -144,6 +150,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   const Tiles tiles(a, r0, nrows);
   const int i0 = (int)((long long)tiles.n * rank / nranks), i1 = (int)((long long)tiles.n * (rank + 1) / nranks);
   const int count = i1 - i0;
+
+  auto fresh = [](int k) { return LONG ? k % FOLD == 0 : k == 0; };  // 16-bit queries: O starts from zero at the k-th tile
 
   if (tid == 0) {
     mbar_init(&q_full, 4);
@@ -236,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           for (int kk = 0; kk < KT / 16; kk++)
             if (kk < 2 || 16 * kk < width)
               mma_ts(d, p + 32 * (kk >> 1) + 8 * (kk & 1) + (PAIR && h == 0 ? 16 : 0), v + kk * (2048 >> 4), IDESC_PV,
-                     h || kk ? 1u : (!PAIR && k > 0));
+                     h || kk ? 1u : (!PAIR && !fresh(k)));
         // The scores of the tile after next take the place of these weights: MMAs run in order. Its commit goes first
         // where O is rarely waited for (a commit costs the issuing warp ~200 cycles).
         if (PAIR) commit(&o_full[st]);
@@ -305,6 +313,30 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
         }
       }
     };
+    // LONG: every FOLD tiles O moves, before it starts from zero again, into the running output of the tiles
+    // before, which is rarely touched and lies in local memory, with the maximum that it is relative to behind it
+    float far[LONG ? D + 1 : 1];
+    far[LONG ? D : 0] = -INFINITY;
+    auto move_far = [&](bool empty) {
+      const float by = far[D] == -INFINITY ? 0.f : exp2_fast(far[D] - m);
+#pragma unroll 1
+      for (int c = 0; c < D / 32; c++) {
+        uint32_t v[32];
+        tmem_ld32(obase + 32 * c, v);
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          far[32 * c + e] = empty ? __uint_as_float(v[e]) : fmaf(far[32 * c + e], by, __uint_as_float(v[e]));
+      }
+      far[D] = m;
+    };
+    auto add_far = [&](int c, uint32_t(&v)[32]) {
+      if constexpr (LONG)
+        if (count > FOLD) {
+          const float by = far[D] == -INFINITY ? 0.f : exp2_fast(far[D] - m);
+#pragma unroll
+          for (int e = 0; e < 32; e++) v[e] = __float_as_uint(fmaf(far[32 * c + e], by, __uint_as_float(v[e])));
+        }
+    };
     for (int k = 0; k < count; k++) {
       const int i = i0 + k;
       if (ok) ok = mbar_wait(&s_full[k % F::RING], (k / F::RING) & 1, nullptr);
@@ -351,11 +383,17 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           }
       }
       mx = mx * sc - TOP<T>;
+      if constexpr (LONG)
+        if (k > 0 && fresh(k)) {
+          wait_o(k - 1);
+          __syncwarp();
+          move_far(k == FOLD);
+        }
       float alpha = 1.f;
       if (PAIR || __any_sync(0xffffffffu, mx > m + GROWTH)) {
         const float mn = fmaxf(m, mx);
         alpha = m == -INFINITY ? 0.f : exp2_fast(m - mn);
-        if (!PAIR && k > 0) {
+        if (!PAIR && !fresh(k)) {
           wait_o(k - 1);
           __syncwarp();
 #pragma unroll
@@ -424,6 +462,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
             for (int e = 0; e < 32; e++) v[e] = __float_as_uint(o[32 * c + e]);
           } else {
             tmem_ld32(obase + 32 * c, v);
+            add_far(c, v);
           }
           const int col = 32 * c;
           if (live) {
@@ -463,6 +502,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
             for (int e = 0; e < 32; e++) v[e] = __float_as_uint(o[32 * c + e]);
           } else {
             tmem_ld32(obase + 32 * c, v);
+            add_far(c, v);
           }
           if (row < nrows) {
             const uint32_t to = peer(&so[at * F::STRIDE + 32 * c], row % nranks);
@@ -528,27 +568,25 @@ int split(int blocks, int tiles) {
   return n;
 }
 
-template <int T, int D>
-cudaError_t launch(Rows a, const void* k, const void* v, int ctx, int tiles, cudaStream_t s) {
+template <int T, int D, bool LONG>
+cudaError_t launch(const Rows& a, const void* k, const void* v, int ctx, cudaStream_t s) {
   using F = Cfg<T, D>;
   CUtensorMap mk, mv;
   cudaError_t e = map_cache(&mk, k, a.kv_heads, ctx, D, KT);
   if (e == cudaSuccess) e = map_cache(&mv, v, a.kv_heads, ctx, D, KT);
   if (e != cudaSuccess) return e;
-  auto* f = k_rows<T, D>;
+  auto* f = k_rows<T, D, LONG>;
   static unsigned long long done = 0;
   static std::mutex mu;
   once_per_device(done, mu, [f] { cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM); });
-  const int blocks = (a.rows + ROWS - 1) / ROWS;
-  const int nranks = a.nranks = split(blocks * a.kv_heads, tiles);
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3((unsigned)nranks * a.kv_heads * blocks);
+  c.gridDim = dim3((unsigned)a.nranks * a.kv_heads * ((a.rows + ROWS - 1) / ROWS));
   c.blockDim = dim3(THREADS);
   c.dynamicSmemBytes = F::SMEM;
   c.stream = s;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = nranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = a.nranks, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // the kernel waits for what is before it (pdl_wait)
   at[1].val.programmaticStreamSerializationAllowed = 1;
   c.attrs = at;
@@ -556,12 +594,24 @@ cudaError_t launch(Rows a, const void* k, const void* v, int ctx, int tiles, cud
   return cudaLaunchKernelEx(&c, f, mk, mv, a);
 }
 
-cudaError_t by_type(int type, int d, const Rows& a, const void* k, const void* v, int ctx, int tiles, cudaStream_t s) {
-  if (type == T_F32)
-    return d == 64 ? launch<T_F32, 64>(a, k, v, ctx, tiles, s) : launch<T_F32, 128>(a, k, v, ctx, tiles, s);
-  if (type == T_F16)
-    return d == 64 ? launch<T_F16, 64>(a, k, v, ctx, tiles, s) : launch<T_F16, 128>(a, k, v, ctx, tiles, s);
-  return d == 64 ? launch<T_BF16, 64>(a, k, v, ctx, tiles, s) : launch<T_BF16, 128>(a, k, v, ctx, tiles, s);
+// `tiles` is the number of position tiles of the last block of rows, which has the most. The fold's own instructions
+// cost 3% where nothing is folded (8192 tokens behind a window of 1500: 209 instead of 203 us).
+cudaError_t by_type(int type, int d, Rows a, const void* k, const void* v, int ctx, int tiles, cudaStream_t s) {
+  a.nranks = split((a.rows + ROWS - 1) / ROWS * a.kv_heads, tiles);
+  const bool lng = (tiles + a.nranks - 1) / a.nranks > FOLD;
+  auto with = [&](auto t, auto d) {
+    constexpr int T = decltype(t)::value, D = decltype(d)::value;
+    if constexpr (T == T_F32)
+      return launch<T, D, false>(a, k, v, ctx, s);
+    else
+      return lng ? launch<T, D, true>(a, k, v, ctx, s) : launch<T, D, false>(a, k, v, ctx, s);
+  };
+  using I = std::integral_constant<int, 64>;
+  using J = std::integral_constant<int, 128>;
+  auto with_d = [&](auto t) { return d == 64 ? with(t, I()) : with(t, J()); };
+  return type == T_F32   ? with_d(std::integral_constant<int, T_F32>())
+         : type == T_F16 ? with_d(std::integral_constant<int, T_F16>())
+                         : with_d(std::integral_constant<int, T_BF16>());
 }
 
 size_t up16(size_t n) { return (n + 15) / 16 * 16; }

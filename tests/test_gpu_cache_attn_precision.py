@@ -109,6 +109,13 @@ def long_reference(q, k, v, heads):
     return out.reshape(-1, heads, d)
 
 
+def mean_error(out, want):
+    """Relative to the 64-bit value, of the distance from that value rounded to the output's type: near a power of two,
+    which the outputs straddle, the steps above are twice those below, so that rounding alone has a mean that is not 0
+    (outputs of mean 1 and deviation s: -(2^-23 - 2^-25) / (s sqrt(2 pi)) in fp16)."""
+    return ((out.double().view_as(want) - want.to(out.dtype).double()) / want).mean().item()
+
+
 # What a long sum may lose in the mean of all outputs. fp32 queries: a tile or chunk of up to eight sums cut off by less
 # than 2^-23 each. fp16: the same up to a fold, 256 sums on the way up to the value, half a step of 2^-23 lost in the mean
 # of each, and six standard deviations of the mean of `count` roundings to fp16 (uniform in half a step of 2^-11).
@@ -123,6 +130,44 @@ def test_long_sums_of_one_token(cuda_lib, kind, heads, kv, n, d, batch):
     every = [x[None].expand(batch, kv, n, d).contiguous() for x in (k, v)]
     out = decode(cuda_lib, kind, heads, q, *every, [n] * batch)
     want = long_reference(q, k, v, heads)
-    bias = ((out.double().view_as(want) - want) / want).mean().item()
+    bias = mean_error(out, want)
     assert status_of(cuda_lib) == 0
     assert abs(bias) <= most_bias(kind, want.numel()), bias
+
+
+@pytest.mark.parametrize("kind,heads,kv,n,d", [("f32", 8, 1, 1 << 18, 64), ("f16", 8, 1, 1 << 20, 64),
+                                               ("f16", 8, 1, 1 << 20, 128)])
+def test_long_sums_of_many_rows(cuda_lib, kind, heads, kv, n, d):
+    """The prompt's last rows and the rows behind a shared prefix, over so many tiles that each CTA folds."""
+    q, k, v = long_rows(n, kind, heads, kv, n, d, 3)
+    want = long_reference(q, k, v, heads)
+    empty = [x[None, :, :1].expand(3, kv, 1, d).contiguous() for x in (k, v)]
+    out = shared(cuda_lib, kind, heads, q, k, v, *empty, [0, 0, 0])
+    bias = mean_error(out, want)
+    assert abs(bias) <= most_bias(kind, want.numel()), bias
+    out = window(cuda_lib, kind, heads, q, k, v, n - 3)[2]  # of the three rows, the one that sees all
+    bias = mean_error(out, want[2])
+    assert abs(bias) <= most_bias(kind, want[2].numel()), bias
+    assert status_of(cuda_lib) == 0
+
+
+@pytest.mark.parametrize("kind,d", [("f16", 64), ("bf16", 128)])
+def test_a_maximum_that_rises_across_folds(cuda_lib, kind, d):
+    """Scores that grow along the positions: outputs folded early are relative to maxima that later ones outgrow, by
+    little (the maximum is not raised) and by much."""
+    import torch
+    heads, kv, n = 4, 1, 70000
+    g = torch.Generator(device="cuda").manual_seed(d)
+    qt, ct = torch_types(kind)
+    q = torch.randn(1, heads * d, generator=g, device="cuda").to(qt)
+    for rise in (3.0, 40.0):
+        x = q.double().view(heads, d)[0]
+        k = 0.3 * torch.randn(kv, n, d, generator=g, device="cuda", dtype=torch.float64)
+        k[0] += torch.linspace(0, rise, n, device="cuda", dtype=torch.float64)[:, None] * x * d ** 0.5 / (x @ x)
+        k, v = k.to(ct), torch.randn(kv, n, d, generator=g, device="cuda").to(ct)
+        out = window(cuda_lib, kind, heads, q, k, v, n - 1)
+        assert status_of(cuda_lib) == 0
+        for h in range(heads):
+            error, most = row_errors(kind, f64(q.cpu()).reshape(heads, d)[h:h + 1], f64(k.cpu()), f64(v.cpu()),
+                                     f64(out.cpu()).reshape(heads, d)[h:h + 1], 8.0)
+            assert error <= most, (rise, h, error, most)
