@@ -362,7 +362,7 @@ lfm_status lfm_attention_prefill(const float* q_dev, uint32_t q_stride, const vo
  * call says so. What a kernel
  * finds wrong in device-side arguments it skips and reports through
  * lfm_attention_status. */
-#define LFM_ATTN_F32 0u  /* fp32 q and out over fp16 caches (the engine's); |q| * scale < 45000 */
+#define LFM_ATTN_F32 0u  /* fp32 q and out over fp16 caches (the engine's) */
 #define LFM_ATTN_F16 1u  /* fp16 q, out and caches */
 #define LFM_ATTN_BF16 2u /* bf16 q, out and caches */
 #define LFM_ATTN_MAX_GROUP 8u

@@ -55,6 +55,30 @@ struct Types<T_BF16> {
 template <int T>
 constexpr float SHIFT = T == T_BF16 ? 0.f : 15.f;
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// fp32 queries enter a product as fp16 hi/lo pairs. A row whose largest value is
+// `most` is multiplied by x, a power of two that brings it to [2^13, 2^14), and
+// its scores by y = 1 / x: both exact, so rows of any size keep the pair's 22
+// bits (without it queries of 1e-3 against keys of 1e3 lost 1e-4 of the output,
+// and those of 65504 and above were infinite). 0, infinities and NaN stay.
+__device__ __forceinline__ float2 row_scale(float most) {
+  int e = __float_as_uint(most) >> 23 & 255;
+  e = e == 255 ? 127 + 13 : max(e, 27);
+  return make_float2(__uint_as_float((unsigned)(2 * 127 + 13 - e) << 23), __uint_as_float((unsigned)(e - 13) << 23));
+}
+template <int N>
+__device__ __forceinline__ float max_abs(const float (&f)[N]) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) m = max3(m, fabsf(f[i]), fabsf(f[i + 1]));
+  return m;
+}
+
 __device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
 __device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
@@ -91,14 +115,14 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 

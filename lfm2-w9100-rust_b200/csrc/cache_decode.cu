@@ -22,7 +22,7 @@
 //       lane reads the same 16 bytes of 4 positions and pairs them by byte
 //       permutes; output column n of tile e is head_dim index 8 n + e.
 // Statistics and outputs stay in fp32; exponentials are of powers of two (the
-// queries or the scores carry scale * log2 e), relative to the maximum less
+// scores carry scale * log2 e), relative to the maximum less
 // SHIFT (cache_common.cuh). 16-bit queries: the weights are rounded to the
 // caches' type, half a step each (fp16 2^-11, bf16 2^-8), as the caller's V and
 // output are; pairs would double the products. The sums l are of the weights as
@@ -134,24 +134,36 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_of(WARPS)) k_decode(Decode a,
   // the query fragments: k step 2 s of head_dim segment [32 s, 32 s + 32) takes a lane's values 0-3 of 8, step 2 s + 1 the others
   constexpr bool PAIR = T == T_F32;
   uint32_t qf[D / 16][4];
-  const float post = PAIR ? 1.f : a.scale * LOG2E;
+  float post = a.scale * LOG2E;
   {
     const Q* q = (const Q*)a.q + (size_t)b * a.q_stride + (size_t)(kh * g + min(r, g - 1)) * D + 8 * t;
+    if constexpr (PAIR) {
+      float f[D / 32][8], most = 0.f;
 #pragma unroll
-    for (int s = 0; s < D / 32; s++) {
-      if constexpr (PAIR) {
+      for (int s = 0; s < D / 32; s++) {
         const float4 x = *(const float4*)(q + 32 * s), y = *(const float4*)(q + 32 * s + 4);
-        const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        f[s][0] = x.x, f[s][1] = x.y, f[s][2] = x.z, f[s][3] = x.w;
+        f[s][4] = y.x, f[s][5] = y.y, f[s][6] = y.z, f[s][7] = y.w;
+        most = fmaxf(most, max_abs(f[s]));
+      }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const float2 by = row_scale(most);
+      post *= by.y;
+#pragma unroll
+      for (int s = 0; s < D / 32; s++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float u = f[2 * i] * (a.scale * LOG2E), v = f[2 * i + 1] * (a.scale * LOG2E);
+          const float u = f[s][2 * i] * by.x, v = f[s][2 * i + 1] * by.x;
           const __half2 h = __floats2half2_rn(u, v);
           const float2 back = __half22float2(h);
           const __half2 l = __floats2half2_rn(u - back.x, v - back.y);
           qf[2 * s + (i >> 1)][(i & 1) * 2] = *(const uint32_t*)&h;
           qf[2 * s + (i >> 1)][(i & 1) * 2 + 1] = *(const uint32_t*)&l;
         }
-      } else {
+    } else {
+#pragma unroll
+      for (int s = 0; s < D / 32; s++) {
         const uint4 x = *(const uint4*)(q + 32 * s);
         const uint32_t f[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_of(WARPS)) k_decode(Decode a,
       }
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const float v = PAIR ? c[e] + c[e + 2] : c[e] * post;
+        const float v = (PAIR ? c[e] + c[e + 2] : c[e]) * post;
         s[kt][e] = i0 + kt * 8 + 2 * t + e < n ? v : -INFINITY;
       }
     }

@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   // may wait for a product when the next one is done too.
   __shared__ uint64_t q_full, k_full[F::RING], v_full[F::RING], s_full[F::RING], o_full[F::RING], p_full[2];
   __shared__ uint32_t tmem_at;
+  __shared__ float s_row[PAIR ? ROWS : 1];  // fp32 queries: what makes a row's scores powers of two
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // blockIdx.x counts ranks, then KV heads, then row tiles, the longest rows first
   const int nranks = a.nranks, rank = blockIdx.x % nranks, kh = blockIdx.x / nranks % a.kv_heads;
@@ -270,14 +271,10 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
         uint8_t* chunk = smem + (c >> 3) * F::Q_CHUNK;
         if constexpr (PAIR) {
           const float4 u = *(const float4*)q, v = *(const float4*)(q + 4);
-          const float f[8] = {u.x * a.scale2, u.y * a.scale2, u.z * a.scale2, u.w * a.scale2,
-                              v.x * a.scale2, v.y * a.scale2, v.z * a.scale2, v.w * a.scale2};
+          const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
           uint32_t h[4], l[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            h[e] = pack(__half(), f[2 * e], f[2 * e + 1]);
-            l[e] = rest(h[e], f[2 * e], f[2 * e + 1]);
-          }
+          const float back = pairs<D / 8>(f, h, l);
+          if (c == 0) s_row[qr] = back * a.scale2;
           st_piece(chunk, qr, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
           st_piece(chunk + F::Q_TILE, qr, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
         } else {
@@ -287,10 +284,11 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
+      if (PAIR) asm volatile("bar.sync 1, 128;" ::: "memory");  // s_row
     }
     const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t obase = mine + COL_O;
-    const float sc = PAIR ? 1.f : a.scale2;
+    const float sc = PAIR ? s_row[PAIR ? row : 0] : a.scale2;
     const int p = a.start + tok;
     const int wlo = a.window > 0 ? p - a.window + 1 : -0x40000000;
     float m = -INFINITY, l = 0.f, alpha_last = 0.f;

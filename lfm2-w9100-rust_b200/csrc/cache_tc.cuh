@@ -57,6 +57,25 @@ __device__ __forceinline__ uint32_t rest(uint32_t hi, float a, float b) {
   const float2 back = __half22float2(*(const __half2*)&hi);
   return pack(__half(), a - back.x, b - back.y);
 }
+// N values of a row that LANES neighbouring lanes of a converged warp share, as fp16 pairs of the row brought to size;
+// returns what brings its scores back.
+template <int LANES, int N>
+__device__ __forceinline__ float pairs(const float (&f)[N], uint32_t (&h)[N / 2], uint32_t (&l)[N / 2]) {
+  float most = max_abs(f);
+#pragma unroll
+  for (int o = 1; o < LANES; o *= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const float2 by = row_scale(most);
+  const uint64_t by2 = two(by.x, by.x), minus = two(-1.f, -1.f);
+#pragma unroll
+  for (int e = 0; e < N / 2; e++) {
+    const uint64_t x = mul2(two(f[2 * e], f[2 * e + 1]), by2);
+    const float2 y = one(x);
+    h[e] = pack(__half(), y.x, y.y);
+    const float2 back = __half22float2(*(const __half2*)&h[e]), z = one(fma2(two(back.x, back.y), minus, x));
+    l[e] = pack(__half(), z.x, z.y);
+  }
+  return by.y;
+}
 // 16 bytes at column block `piece` (of 8) of row r of a swizzled 64-wide chunk
 __device__ __forceinline__ void st_piece(uint8_t* chunk, int r, int piece, uint4 v) {
   *(uint4*)(chunk + r * 128 + ((piece ^ (r & 7)) << 4)) = v;

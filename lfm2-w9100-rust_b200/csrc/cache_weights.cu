@@ -18,7 +18,8 @@
 // degree 5) took the units' time down to 55% and left the total: the issuing warp
 // and the sums' start on each tile are what is left. Tiles of 128 rows in four buffers: 350 us;
 // eight warps for the sums: 434 us. fp32 queries are bound by making their pairs, once for each tile
-// of keys: 3840 tokens of 32 heads and 64 values 182 us with eight warps at it, 385 us with four.
+// of keys: 3840 tokens of 32 heads and 64 values 170 us with eight warps at it (four: 385 before the pairs were made two
+// pieces at a time).
 // A key is summed by one thread, in the order of the rows, tile by tile, and the
 // CTAs of a cluster that splits the rows are added up in their order: the
 // result is the same on every run.
@@ -71,6 +72,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
   __shared__ uint64_t k_full, full[F::RING], empty[F::RING], s_full[2], s_free[2], lse_full[LSE_RING], lse_free[LSE_RING];
   __shared__ uint32_t tmem_at;
   __shared__ __align__(16) float s_lse[LSE_RING][F::N];  // -lse in log2 units
+  __shared__ __align__(16) float s_row[LSE_RING][PAIR ? F::N : 4];  // fp32 queries: what makes a row's scores powers of two
   __shared__ float s_sum[8][KEYS];                      // the quarters' sums, then those of the cluster's CTAs
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // blockIdx.x counts ranks, then KV heads, then tiles: the first keys, which most rows see, come first
@@ -158,8 +160,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
     // --------------------------------------------------------------- sums
     constexpr int COLS = F::N / PARTS;
     const int part = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane, j = j0 + key;
-    const float sc = PAIR ? 1.f : a.scale2;
-    const uint64_t sc2 = two(sc, sc);
+    const uint64_t sc2 = two(a.scale2, a.scale2);
     for (int k = 0; k < count; k++) {
       if (!(ok = mbar_wait(&lse_full[k % LSE_RING], (k / LSE_RING) & 1, nullptr) &&
                  mbar_wait(&s_full[k & 1], (k >> 1) & 1, nullptr)))
@@ -178,6 +179,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
       }
       const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16) + 256 * (k & 1) + part * COLS;
       const float* nl = s_lse[k % LSE_RING] + part * COLS;
+      const float* rs = s_row[k % LSE_RING] + (PAIR ? part * COLS : 0);
       uint64_t s2[2] = {0, 0};  // pairs of 0.f
 #pragma unroll
       for (int c = 0; c < COLS / 32; c++) {
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
           if (__any_sync(0xffffffffu, see != 0)) {
 #pragma unroll
             for (int e = 0; e < 32; e++) {
-              const float x = exp2_fast(fmaf(__uint_as_float(w[e]), sc, nl[32 * c + e]));
+              const float x = exp2_fast(fmaf(__uint_as_float(w[e]), PAIR ? rs[32 * c + e] : a.scale2, nl[32 * c + e]));
               if (see >> e & 1) sum += x;
             }
           }
@@ -198,7 +200,12 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
 #pragma unroll
         for (int e = 0; e < 16; e++) {
           const float4 n4 = ((const float4*)(nl + 32 * c))[e / 2];
-          const uint64_t x = fma2(two(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1])), sc2,
+          uint64_t by = sc2;
+          if constexpr (PAIR) {
+            const float4 r4 = ((const float4*)(rs + 32 * c))[e / 2];
+            by = e & 1 ? two(r4.z, r4.w) : two(r4.x, r4.y);
+          }
+          const uint64_t x = fma2(two(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1])), by,
                                   e & 1 ? two(n4.z, n4.w) : two(n4.x, n4.y));
           const float2 y = one(x);
           s2[e & 1] = add2(s2[e & 1], two(exp2_fast(y.x), exp2_fast(y.y)));
@@ -247,26 +254,30 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
       if constexpr (PAIR) {
         if (k >= F::RING && !(ok = mbar_wait(&empty[st], (k / F::RING - 1) & 1, nullptr))) return;
         uint8_t* dst = smem + F::K_TILE + st * F::STAGE;
-#pragma unroll 2
-        for (int i = ft; i < cols * (D / 8); i += 32 * F::FEED) {
-          const int row = i / (D / 8), c = i % (D / 8);
-          float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
+        constexpr int LANES = D / 16;  // to a row, each with the 8-value pieces c and c + LANES
+#pragma unroll 1
+        for (int i = ft; i < cols * LANES; i += 32 * F::FEED) {
+          const int row = i / LANES, c = i % LANES;
+          float f[16] = {};
           if (row < have) {
             const int t = row * per_row >> 16;
             const float* q = a.q + (size_t)(t0 + t) * a.q_stride + (size_t)(kh * a.g + row - t * a.g) * D + 8 * c;
-            u = *(const float4*)q, w = *(const float4*)(q + 4);
-          }
-          const float f[8] = {u.x * a.scale2, u.y * a.scale2, u.z * a.scale2, u.w * a.scale2,
-                              w.x * a.scale2, w.y * a.scale2, w.z * a.scale2, w.w * a.scale2};
-          uint32_t h[4], l[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            h[e] = pack(__half(), f[2 * e], f[2 * e + 1]);
-            l[e] = rest(h[e], f[2 * e], f[2 * e + 1]);
+            for (int e = 0; e < 4; e++) {
+              const float4 u = *(const float4*)(q + (e >> 1) * 8 * LANES + (e & 1) * 4);
+              f[4 * e] = u.x, f[4 * e + 1] = u.y, f[4 * e + 2] = u.z, f[4 * e + 3] = u.w;
+            }
           }
-          uint8_t* chunk = dst + (c >> 3) * F::Q_CHUNK;
-          st_piece(chunk, row, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
-          st_piece(chunk + F::Q_TILE, row, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
+          uint32_t h[8], l[8];
+          const float back = pairs<LANES>(f, h, l);
+          if (c == 0) s_row[k % LSE_RING][row] = back * a.scale2;
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int piece = c + e * LANES;
+            uint8_t* chunk = dst + (piece >> 3) * F::Q_CHUNK;
+            st_piece(chunk, row, piece & 7, make_uint4(h[4 * e], h[4 * e + 1], h[4 * e + 2], h[4 * e + 3]));
+            st_piece(chunk + F::Q_TILE, row, piece & 7, make_uint4(l[4 * e], l[4 * e + 1], l[4 * e + 2], l[4 * e + 3]));
+          }
         }
         fence_async_smem();
       }

@@ -171,3 +171,44 @@ def test_a_maximum_that_rises_across_folds(cuda_lib, kind, d):
             error, most = row_errors(kind, f64(q.cpu()).reshape(heads, d)[h:h + 1], f64(k.cpu()), f64(v.cpu()),
                                      f64(out.cpu()).reshape(heads, d)[h:h + 1], 8.0)
             assert error <= most, (rise, h, error, most)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_fp32_queries_of_any_size(cuda_lib, d):
+    """Rows of one call whose queries differ by many orders of magnitude, against keys of the inverse size: fp32 holds
+    them all alike. One KV head to a size."""
+    import torch
+    sizes = [1e-4, 1e-2, 1.0, 40.0, 3e5]
+    kv, n, g = len(sizes), 400, 2
+    heads, rng = g * kv, np.random.default_rng(d)
+    x = (rng.normal(0, 1, (heads, d)) * np.repeat(sizes, g)[:, None]).astype(np.float32)
+    k = (rng.normal(0, 1, (kv, n, d)) / np.array(sizes)[:, None, None]).astype(np.float16)
+    v = rng.normal(0, 1, (kv, n, d)).astype(np.float16)
+    assert np.isfinite(k).all()
+    x, k, v = x.astype(np.float64), k.astype(np.float64), v.astype(np.float64)
+    qd, kd, vd = on_gpu(x.reshape(1, -1), "f32", False), on_gpu(k, "f32", True), on_gpu(v, "f32", True)
+    empty = kd[None, :, :1].contiguous(), vd[None, :, :1].contiguous()
+    acc, lse = torch.zeros(1, kv, n, device="cuda"), torch.zeros(1, heads, device="cuda")
+    outs = {"decode": decode(cuda_lib, "f32", heads, qd, kd[None], vd[None], [n], acc),
+            "window": window(cuda_lib, "f32", heads, qd, kd, vd, n - 1, lse),
+            "shared": shared(cuda_lib, "f32", heads, qd, kd, vd, *empty, [0])}
+    for name, out in outs.items():
+        got = f64(out.cpu()).reshape(heads, d)
+        for h in range(kv):
+            rows = slice(h * g, (h + 1) * g)
+            error, most = row_errors("f32", x[rows], k[h:h + 1], v[h:h + 1], got[rows])
+            assert error <= most, (name, sizes[h], error, most)
+    acc2 = torch.zeros(kv, n, device="cuda")
+    check(cuda_lib.lfm_attention_weights(shape_of("f32", heads, kv, d, n), ptr(qd), heads * d, ptr(kd), n - 1, 1, 0, 0,
+                                         ptr(lse), ptr(acc2), None), "weights")
+    assert status_of(cuda_lib) == 0
+    for h in range(kv):
+        s = x[h * g:(h + 1) * g] @ k[h].T * d ** -0.5
+        w = np.exp(s - s.max(1, keepdims=True))
+        want = (w / w.sum(1, keepdims=True)).sum(0)
+        s32 = (x[h * g:(h + 1) * g].astype(np.float32) @ k[h].T.astype(np.float32)) * np.float32(d ** -0.5)
+        w32 = np.exp(s32 - s32.max(1, keepdims=True))
+        plain = norm_error((w32 / w32.sum(1, keepdims=True)).sum(0), want)
+        most = limit("f32", plain, score_cut(d, s))
+        for got in (acc[0, h], acc2[h]):
+            assert norm_error(f64(got.cpu()), want) <= most, (sizes[h], norm_error(f64(got.cpu()), want), most)
