@@ -95,19 +95,23 @@ __global__ void __launch_bounds__(THREADS, 4) k_evict(Evict a, bool in_place) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
       for (int i = tid; i < BINS; i += THREADS) u.hist[i] = 0;
       __syncthreads();
+      // a warp's 32 neighbours together, those behind the last too: every lane takes part in the warp's votes
 #pragma unroll 8
-      for (int i = lo + tid; i < hi; i += THREADS) {
-        const unsigned k = key_of(i);
-        if ((k & known) != T) continue;
+      for (int first = lo + tid - lane; first < hi; first += THREADS) {
+        const int i = first + lane;
+        const unsigned k = i < hi ? key_of(i) : 0u;
         const int bin = k >> shift & ((1 << bits) - 1);
-        // equal weights are common (positions never looked at): one addition for a warp's
-        int same;
-        const unsigned m = __activemask();
-        __match_all_sync(m, bin, &same);
-        if (!same)
-          atomicAdd(&u.hist[bin], 1);
-        else if (lane == __ffs(m) - 1)
-          atomicAdd(&u.hist[bin], __popc(m));
+        const bool counts = i < hi && (k & known) == T;
+        // equal weights are common (positions never looked at): one addition for those of a warp
+        const unsigned members = __ballot_sync(0xffffffffu, counts);
+        if (counts) {
+          int same;
+          __match_all_sync(members, bin, &same);
+          if (!same)
+            atomicAdd(&u.hist[bin], 1);
+          else if (lane == __ffs(members) - 1)
+            atomicAdd(&u.hist[bin], __popc(members));
+        }
       }
       __syncthreads();
       // from the highest bin down: the one with the `ties`-th key
