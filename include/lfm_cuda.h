@@ -446,7 +446,10 @@ lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const
 /* Waits for `stream` and returns what the calls above have reported on the
  * current device since the last call of this one, as the sum of LFM_ATTN_BAD_*;
  * 0: nothing. A device-side wait that ran out (about a second) reports
- * LFM_ATTN_BAD_WAIT; the results of the calls since then are not to be used. */
+ * LFM_ATTN_BAD_WAIT; the results of the calls since then are not to be used.
+ * A report that another stream's call makes meanwhile is returned by this call
+ * or by the next. Refused while `stream` is captured. On an error *status is
+ * left as it was. */
 #define LFM_ATTN_BAD_WAIT 1u
 #define LFM_ATTN_BAD_SLOT 2u
 #define LFM_ATTN_BAD_LEN 4u

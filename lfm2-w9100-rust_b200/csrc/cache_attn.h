@@ -69,11 +69,11 @@ cudaError_t decode_joined(const Decode& a, const float* o, const float2* ml, cud
 size_t shared_workspace(const Decode& a);
 cudaError_t shared(const Decode& a, cudaStream_t s);
 cudaError_t evict(const Evict& a, cudaStream_t s);
-// Adds what the kernels of each file have reported on this device to *bits and clears it; waits for the stream.
-cudaError_t take_status_tc(unsigned* bits, cudaStream_t s);
-cudaError_t take_status_weights(unsigned* bits, cudaStream_t s);
-cudaError_t take_status_decode(unsigned* bits, cudaStream_t s);
-cudaError_t take_status_evict(unsigned* bits, cudaStream_t s);
+// Where the kernels of each file report on the current device.
+cudaError_t status_word_tc(unsigned** at);
+cudaError_t status_word_weights(unsigned** at);
+cudaError_t status_word_decode(unsigned** at);
+cudaError_t status_word_evict(unsigned** at);
 
 }  // namespace cache
 }  // namespace lfm

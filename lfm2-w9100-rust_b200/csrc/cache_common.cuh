@@ -15,15 +15,7 @@ static __device__ unsigned g_status;
 __device__ __forceinline__ void report(unsigned bits) { atomicOr(&g_status, bits); }
 
 // (static, like the variable: each file has its own)
-static cudaError_t take_status(unsigned* bits, cudaStream_t s) {
-  unsigned *at = nullptr, got = 0;
-  cudaError_t e = cudaGetSymbolAddress((void**)&at, g_status);
-  if (e == cudaSuccess) e = cudaMemcpyAsync(&got, at, sizeof got, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaMemsetAsync(at, 0, sizeof got, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  *bits |= got;
-  return e;
-}
+static cudaError_t status_word(unsigned** at) { return cudaGetSymbolAddress((void**)at, g_status); }
 
 // The element types of LFM_ATTN_*: q and out, and the caches.
 template <int T>

@@ -472,7 +472,7 @@ cudaError_t decode_joined(const Decode& a, const float* o, const float2* ml, cud
   return run(a, Joint{o, ml}, s);
 }
 
-cudaError_t take_status_decode(unsigned* bits, cudaStream_t s) { return take_status(bits, s); }
+cudaError_t status_word_decode(unsigned** at) { return status_word(at); }
 
 }  // namespace cache
 }  // namespace lfm

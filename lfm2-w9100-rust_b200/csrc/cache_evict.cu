@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(THREADS, 4) k_evict(Evict a, bool in_place) {
 }
 }  // namespace
 
-cudaError_t take_status_evict(unsigned* bits, cudaStream_t s) { return take_status(bits, s); }
+cudaError_t status_word_evict(unsigned** at) { return status_word(at); }
 
 cudaError_t evict(const Evict& a, cudaStream_t s) {
   // As many CTAs to a head as give every SM two, each with a round of its own at least. More repeat the selection for

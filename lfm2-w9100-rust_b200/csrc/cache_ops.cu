@@ -4,6 +4,8 @@
 #include <math.h>
 #include <stdio.h>
 
+#include <mutex>
+
 #include "../../include/lfm_cuda.h"
 #include "cache_attn.h"
 #include "kernels.h"
@@ -119,6 +121,12 @@ lfm_status decode_args(const char* who, const lfm_attn_shape* s, const void* q, 
 bool decode_here(const Decode& a) {
   return here(a.q) && here(a.k) && here(a.v) && here(a.lens) && here(a.out) && (!a.slots || here(a.slots)) &&
          (!a.acc || here(a.acc));
+}
+
+// What has been reported is taken and cleared in one step of each word: kernels of other streams report meanwhile.
+__device__ unsigned g_taken;
+__global__ void k_take(unsigned* a, unsigned* b, unsigned* c, unsigned* d) {
+  g_taken = atomicExch(a, 0u) | atomicExch(b, 0u) | atomicExch(c, 0u) | atomicExch(d, 0u);
 }
 
 struct Range {
@@ -258,12 +266,26 @@ lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const
 lfm_status lfm_attention_status(uint32_t* status, void* stream) {
   const char* who = "lfm_attention_status";
   if (!status) return bad(who, "status is null");
-  unsigned bits = 0;
-  cudaError_t e = lfm::cache::take_status_tc(&bits, (cudaStream_t)stream);
-  if (e == cudaSuccess) e = lfm::cache::take_status_weights(&bits, (cudaStream_t)stream);
-  if (e == cudaSuccess) e = lfm::cache::take_status_decode(&bits, (cudaStream_t)stream);
-  if (e == cudaSuccess) e = lfm::cache::take_status_evict(&bits, (cudaStream_t)stream);
-  *status = bits;
+  const cudaStream_t s = (cudaStream_t)stream;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaError_t e = cudaStreamIsCapturing(s, &capture)) return done(who, e);
+  if (capture != cudaStreamCaptureStatusNone) return bad(who, "waits for the stream, which is being captured");
+  unsigned *words[4] = {}, *taken = nullptr, bits = 0;
+  cudaError_t e = lfm::cache::status_word_tc(&words[0]);
+  if (e == cudaSuccess) e = lfm::cache::status_word_weights(&words[1]);
+  if (e == cudaSuccess) e = lfm::cache::status_word_decode(&words[2]);
+  if (e == cudaSuccess) e = lfm::cache::status_word_evict(&words[3]);
+  if (e == cudaSuccess) e = cudaGetSymbolAddress((void**)&taken, g_taken);
+  if (e != cudaSuccess) return done(who, e);
+  // one call at a time, to the end of its wait: g_taken is the device's
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  k_take<<<1, 1, 0, s>>>(words[0], words[1], words[2], words[3]);
+  e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&bits, taken, sizeof bits, cudaMemcpyDeviceToHost, s);
+  const cudaError_t waited = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) e = waited;
+  if (e == cudaSuccess) *status = bits;
   return done(who, e);
 }
 

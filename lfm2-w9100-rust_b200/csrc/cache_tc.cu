@@ -647,7 +647,7 @@ cudaError_t shared(const Decode& a, cudaStream_t s) {
   return decode_joined(a, r.part, r.part_ml, s);
 }
 
-cudaError_t take_status_tc(unsigned* bits, cudaStream_t s) { return take_status(bits, s); }
+cudaError_t status_word_tc(unsigned** at) { return status_word(at); }
 
 }  // namespace cache
 }  // namespace lfm

@@ -368,7 +368,7 @@ cudaError_t weights(const Prompt& a, cudaStream_t s) {
   return a.d == 64 ? launch<T_BF16, 64>(a, s) : launch<T_BF16, 128>(a, s);
 }
 
-cudaError_t take_status_weights(unsigned* bits, cudaStream_t s) { return take_status(bits, s); }
+cudaError_t status_word_weights(unsigned** at) { return status_word(at); }
 
 }  // namespace cache
 }  // namespace lfm
