@@ -75,6 +75,13 @@ __device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
 __device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
 __device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
 
+// Bounded waits, false where they ran out. warp_wait is one for the warp: its lanes' limits end apart, and what follows
+// (shuffles, tensor-memory loads) needs all lanes, so they leave it together. lane_wait is for code that one lane alone runs.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, dev::mbar_wait(bar, parity, nullptr));
+}
+__device__ __forceinline__ bool lane_wait(uint64_t* bar, uint32_t parity) { return dev::mbar_wait(bar, parity, nullptr); }
+
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

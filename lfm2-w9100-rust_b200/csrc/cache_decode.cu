@@ -196,9 +196,15 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_of(WARPS)) k_decode(Decode a,
 
   float m = -INFINITY, l = 0.f, o[NU][8][2] = {};  // o: head r, column 64 u + 8 (2 t + x) + e
   bool ok = true;
+  // the k-th fetch has landed; if it does not, the ones behind it are waited for too before their place is given up
+  auto landed = [&](int k, int end) {
+    if (warp_wait(&full[w][k % STAGES], (k / STAGES) & 1)) return true;
+    for (int j = k; j < min(k + STAGES, end); j++) warp_wait(&full[w][j % STAGES], (j / STAGES) & 1);
+    return false;
+  };
   for (int i = 0; i < mine && ok; i++) {
     const int st = i % STAGES, i0 = (c0 + w + i * WARPS) * KC;
-    if (!(ok = mbar_wait(&full[w][st], (i / STAGES) & 1, nullptr))) break;
+    if (!(ok = landed(i, mine))) break;
     uint8_t* kb = ring + st * STAGE;
     uint8_t* vb = kb + HALF;
     if (i0 + KC > n) {  // the rows behind the last hold what was there before: their weights are 0, so they must be finite
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(WARPS * 32, ctas_of(WARPS)) k_decode(Decode a,
           for (int i = 0; i < min(mine, STAGES); i++) fetch(i, (mine + i) % STAGES, false);
         for (int i = 0; i < mine && ok; i++) {
           const int at = mine + i, st = at % STAGES, i0 = (c0 + w + i * WARPS) * KC;
-          if (!(ok = mbar_wait(&full[w][st], (at / STAGES) & 1, nullptr))) break;
+          if (!(ok = landed(at, 2 * mine))) break;
           float s[TILES][2];
           score(ring + st * STAGE, i0, s);
 #pragma unroll

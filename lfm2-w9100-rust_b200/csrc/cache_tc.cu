@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
   // s_full: scores computed, and with them the K tile free again; o_full: output added, and with it the V tile. One of
   // each for every ring place, because a parity must not come round before its last reader has come by: a softmax warp
   // may wait for a product when the next one is done too.
-  __shared__ uint64_t q_full, k_full[F::RING], v_full[F::RING], s_full[F::RING], o_full[F::RING], p_full[2];
+  __shared__ uint64_t q_full, k_full[F::RING], v_full[F::RING], s_full[F::RING], o_full[F::RING], p_full[2], drained;
   __shared__ uint32_t tmem_at;
   __shared__ float s_row[PAIR ? ROWS : 1];  // fp32 queries: what makes a row's scores powers of two
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < 2; i++) mbar_init(&p_full[i], 4);
+    mbar_init(&drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(&tmem_at, COLS);
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       int nk = 0, nv = 0;
       auto load = [&](const CUtensorMap* map, int& k, uint64_t* full, uint64_t* free, int at) {
         const int st = k % F::RING;
-        if (!ok || (k >= F::RING && !(ok = mbar_wait(&free[st], (k / F::RING - 1) & 1, nullptr)))) return;
+        if (!ok || (k >= F::RING && !(ok = lane_wait(&free[st], (k / F::RING - 1) & 1)))) return;
         mbar_expect_tx(&full[st], F::TILE);
 #pragma unroll
         for (int c = 0; c < D / 64; c++)
@@ -194,19 +195,16 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       }
       if (!ok) report(BAD_WAIT);
       // the copies land before the CTA's shared memory is used for anything else
-      for (int k = max(0, nk - F::RING); k < nk; k++) mbar_wait(&k_full[k % F::RING], (k / F::RING) & 1, nullptr);
-      for (int k = max(0, nv - F::RING); k < nv; k++) mbar_wait(&v_full[k % F::RING], (k / F::RING) & 1, nullptr);
+      for (int k = max(0, nk - F::RING); k < nk; k++) lane_wait(&k_full[k % F::RING], (k / F::RING) & 1);
+      for (int k = max(0, nv - F::RING); k < nv; k++) lane_wait(&v_full[k % F::RING], (k / F::RING) & 1);
     } else if (warp == 1 && count > 0) {
       // -------------------------------------------------------------- MMAs
       constexpr uint32_t IDESC_PV = idesc_f16(ROWS, D, true) | BF;
       const uint32_t tm = uniform(tmem), q0 = uniform(smem_u32(smem)), ring0 = uniform(smem_u32(ring));
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, nullptr));
-      };
-      bool ok = wait(&q_full, 0);
+      bool ok = warp_wait(&q_full, 0);
       auto qk = [&](int k) {  // this CTA's k-th tile
         const int st = k % F::RING;
-        if (k >= count || !ok || !(ok = wait(&k_full[st], (k / F::RING) & 1))) return;
+        if (k >= count || !ok || !(ok = warp_wait(&k_full[st], (k / F::RING) & 1))) return;
         tc_fence_after();
         const uint32_t idesc = idesc_f16(ROWS, tiles.width(i0 + k), false) | BF;
         const uint32_t d = tm + KT * (k & 1);
@@ -223,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
       qk(1);
       for (int k = 0; k < count && ok; k++) {
         const int st = k % F::RING;
-        if (!(ok = wait(&v_full[st], (k / F::RING) & 1))) break;
+        if (!(ok = warp_wait(&v_full[st], (k / F::RING) & 1))) break;
         const uint32_t vb = ring0 + (2 * st + 1) * F::TILE;
         const int width = tiles.width(i0 + k), valid = tiles.all(i0 + k) ? KT : tiles.valid(i0 + k);
         if (valid < width) {  // rows that no query sees: their weights are 0, so they must be finite
@@ -235,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           fence_async_smem();
           __syncwarp();
         }
-        if (!(ok = wait(&p_full[k & 1], (k >> 1) & 1))) break;
+        if (!(ok = warp_wait(&p_full[k & 1], (k >> 1) & 1))) break;
         tc_fence_after();
         const uint32_t d = tm + COL_O + D * (k & (F::OBUF - 1)), p = tm + KT * (k & 1);
         const uint64_t v = smem_desc_mn_sw128(vb, F::KV_CHUNK);
@@ -252,7 +250,11 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
         qk(k + 2);
         if (!PAIR) commit(&o_full[st]);
       }
-      if (!ok && lane == 0) report(BAD_WAIT);
+      if (!ok) {
+        commit(&drained);  // no product is left in flight when the tensor memory goes
+        warp_wait(&drained, 0);
+        if (lane == 0) report(BAD_WAIT);
+      }
     }
   } else {
     // -------------------------------------------------------------- softmax
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     float o[PAIR ? D : 1] = {};  // fp32 queries: the running output
     bool ok = true;
     auto wait_o = [&](int k) {  // the k-th product has been added
-      if (ok) ok = mbar_wait(&o_full[k % F::RING], (k / F::RING) & 1, nullptr);
+      if (ok) ok = warp_wait(&o_full[k % F::RING], (k / F::RING) & 1);
       tc_fence_after();
     };
     auto fold = [&](int k) {  // O of the k-th tile, whose maximum came with alpha_last
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
     };
     for (int k = 0; k < count; k++) {
       const int i = i0 + k;
-      if (ok) ok = mbar_wait(&s_full[k % F::RING], (k / F::RING) & 1, nullptr);
+      if (ok) ok = warp_wait(&s_full[k % F::RING], (k / F::RING) & 1);
       if (!ok) break;
       __syncwarp();
       tc_fence_after();

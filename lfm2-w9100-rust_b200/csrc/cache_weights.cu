@@ -69,7 +69,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
   constexpr bool PAIR = F::PAIR;
   constexpr uint32_t BF = std::is_same<C, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
   extern __shared__ __align__(1024) uint8_t smem[];  // K, then the ring of query tiles
-  __shared__ uint64_t k_full, full[F::RING], empty[F::RING], s_full[2], s_free[2], lse_full[LSE_RING], lse_free[LSE_RING];
+  __shared__ uint64_t k_full, full[F::RING], empty[F::RING], s_full[2], s_free[2], lse_full[LSE_RING], lse_free[LSE_RING], drained;
   __shared__ uint32_t tmem_at;
   __shared__ __align__(16) float s_lse[LSE_RING][F::N];  // -lse in log2 units
   __shared__ __align__(16) float s_row[LSE_RING][PAIR ? F::N : 4];  // fp32 queries: what makes a row's scores powers of two
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
 
   if (tid == 0) {
     mbar_init(&k_full, 1);
+    mbar_init(&drained, 1);
     for (int i = 0; i < F::RING; i++) {
       mbar_init(&full[i], PAIR ? F::FEED : 1);
       mbar_init(&empty[i], 1);
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
       if (!PAIR)
         for (; k < count; k++) {
           const int st = k % F::RING;
-          if (k >= F::RING && !(ok = mbar_wait(&empty[st], (k / F::RING - 1) & 1, nullptr))) break;
+          if (k >= F::RING && !(ok = lane_wait(&empty[st], (k / F::RING - 1) & 1))) break;
           mbar_expect_tx(&full[st], cols * 2 * D);
 #pragma unroll
           for (int c = 0; c < D / 64; c++)
@@ -129,21 +130,18 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
                         &full[st]);
         }
       // the copies land before the CTA ends
-      mbar_wait(&k_full, 0, nullptr);
-      for (int i = max(0, k - F::RING); i < k; i++) mbar_wait(&full[i % F::RING], (i / F::RING) & 1, nullptr);
+      lane_wait(&k_full, 0);
+      for (int i = max(0, k - F::RING); i < k; i++) lane_wait(&full[i % F::RING], (i / F::RING) & 1);
     }
   } else if (warp == 1) {
     if (count > 0) {
       const uint32_t tm = uniform(tmem), kb = uniform(smem_u32(smem));
       const uint32_t idesc = idesc_f16(KEYS, cols, false) | BF;
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, nullptr));
-      };
-      ok = wait(&k_full, 0);
+      ok = warp_wait(&k_full, 0);
       for (int k = 0; k < count && ok; k++) {
         const int st = k % F::RING;
-        if (!(ok = wait(&full[st], (k / F::RING) & 1))) break;
-        if (k >= 2 && !(ok = wait(&s_free[k & 1], (k / 2 - 1) & 1))) break;
+        if (!(ok = warp_wait(&full[st], (k / F::RING) & 1))) break;
+        if (k >= 2 && !(ok = warp_wait(&s_free[k & 1], (k / 2 - 1) & 1))) break;
         tc_fence_after();
         const uint64_t kd = smem_desc_sw128(kb), qd = smem_desc_sw128(kb + F::K_TILE + st * F::STAGE);
 #pragma unroll
@@ -155,6 +153,10 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
         commit(&s_full[k & 1]);
         commit(&empty[st]);
       }
+      if (!ok) {
+        commit(&drained);  // no product is left in flight when the tensor memory goes
+        warp_wait(&drained, 0);
+      }
     }
   } else if (warp < 2 + EPI) {
     // --------------------------------------------------------------- sums
@@ -162,8 +164,7 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
     const int part = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane, j = j0 + key;
     const uint64_t sc2 = two(a.scale2, a.scale2);
     for (int k = 0; k < count; k++) {
-      if (!(ok = mbar_wait(&lse_full[k % LSE_RING], (k / LSE_RING) & 1, nullptr) &&
-                 mbar_wait(&s_full[k & 1], (k >> 1) & 1, nullptr)))
+      if (!(ok = warp_wait(&lse_full[k % LSE_RING], (k / LSE_RING) & 1) && warp_wait(&s_full[k & 1], (k >> 1) & 1)))
         break;
       __syncwarp();
       tc_fence_after();
@@ -246,13 +247,13 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
     for (int i = 0; i < AHEAD; i++) fetch(i, pre[i]);
     auto feed = [&](int k, float(&e)[PER]) {
       const int st = k % F::RING, t0 = (i0 + k) * a.tokens, have = min(a.tokens, a.n - t0) * a.g;
-      if (k >= LSE_RING && !(ok = mbar_wait(&lse_free[k % LSE_RING], (k / LSE_RING - 1) & 1, nullptr))) return;
+      if (k >= LSE_RING && !(ok = warp_wait(&lse_free[k % LSE_RING], (k / LSE_RING - 1) & 1))) return;
 #pragma unroll
       for (int i = 0; i < PER; i++)
         if (ft + 32 * F::FEED * i < F::N) s_lse[k % LSE_RING][ft + 32 * F::FEED * i] = -LOG2E * e[i];
       fetch(k + AHEAD, e);
       if constexpr (PAIR) {
-        if (k >= F::RING && !(ok = mbar_wait(&empty[st], (k / F::RING - 1) & 1, nullptr))) return;
+        if (k >= F::RING && !(ok = warp_wait(&empty[st], (k / F::RING - 1) & 1))) return;
         uint8_t* dst = smem + F::K_TILE + st * F::STAGE;
         constexpr int LANES = D / 16;  // to a row, each with the 8-value pieces c and c + LANES
 #pragma unroll 1
