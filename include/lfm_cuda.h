@@ -432,7 +432,8 @@ lfm_status lfm_attention_weights(const lfm_attn_shape* shape, const void* q, uin
  * [kv_heads][ctx] int32, the caller's record of what a cache row holds; may be
  * null), from the source arrays to the same slots of the destination arrays,
  * which are the source arrays themselves (in place; all of them then) or do
- * not overlap them. lens_out[b] = min(lens[b], budget), in another array than
+ * not overlap them (slots of K and of V may lie between one another, as in an
+ * array [slot][K, V][kv_heads][ctx][head_dim]). lens_out[b] = min(lens[b], budget), in another array than
  * lens. Rows behind the kept ones are left as they were. Only dtype's cache type, kv_heads, head_dim and
  * ctx of `shape` are used. Slots are distinct: a session whose slot an earlier
  * one has, or whose slot or length is out of range, is left out and reported

@@ -129,11 +129,22 @@ __global__ void k_take(unsigned* a, unsigned* b, unsigned* c, unsigned* d) {
   g_taken = atomicExch(a, 0u) | atomicExch(b, 0u) | atomicExch(c, 0u) | atomicExch(d, 0u);
 }
 
-struct Range {
-  const char* p;
-  size_t n;
+// `count` blocks of n bytes, `stride` bytes from one to the next; in 128 bits, since n_slots and slot_stride may be
+// anything that an array could not have.
+using Wide = __int128;
+struct Blocks {
+  const void* p;
+  Wide n, stride, count;
 };
-bool overlap(Range a, Range b) { return a.p && b.p && a.p < b.p + b.n && b.p < a.p + a.n; }
+Wide floor_div(Wide a, Wide b) { return a / b - (a % b < 0); }
+// Blocks of one stride (or one block alone): some i - j = k of theirs meet where -b.n < b.p - a.p - k stride < a.n.
+bool overlap(const Blocks& a, const Blocks& b) {
+  if (!a.p || !b.p) return false;
+  const Wide stride = a.count > 1 ? a.stride : b.count > 1 ? b.stride : 1;
+  const Wide d = (Wide)(uintptr_t)b.p - (Wide)(uintptr_t)a.p;
+  const Wide lo = floor_div(d - a.n, stride) + 1, hi = -floor_div(-(d + b.n), stride) - 1;
+  return (lo > 1 - b.count ? lo : 1 - b.count) <= (hi < a.count - 1 ? hi : a.count - 1);
+}
 }  // namespace
 
 extern "C" {
@@ -223,13 +234,13 @@ lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const
   if (const char* e = slots_error(shape, slot_stride, n_slots, slots, lens, batch, max_len)) return bad(who, e);
   if (budget == 0 || (uint64_t)keep_first + keep_last > budget)
     return bad(who, "budget >= 1 and keep_first + keep_last <= budget");
-  const size_t rows = (size_t)shape->kv_heads * shape->ctx;
-  const size_t cache = 2 * ((size_t)(n_slots - 1) * slot_stride + rows * shape->head_dim), per = 4 * rows * n_slots;
-  const Range src[4] = {{(const char*)k_src, cache}, {(const char*)v_src, cache}, {(const char*)acc_src, per},
-                        {(const char*)pos_src, per}};
-  const Range dst[5] = {{(const char*)k_dst, cache}, {(const char*)v_dst, cache}, {(const char*)acc_dst, per},
-                        {(const char*)pos_dst, per}, {(const char*)lens_out, 4 * (size_t)batch}};
-  const Range in[2] = {{(const char*)lens, 4 * (size_t)batch}, {(const char*)slots, 4 * (size_t)batch}};
+  const Wide rows = (Wide)shape->kv_heads * shape->ctx, step = 2 * (Wide)slot_stride;
+  auto slots_of = [&](const void* p) { return Blocks{p, 2 * rows * shape->head_dim, step, n_slots}; };
+  auto records = [&](const void* p) { return Blocks{p, 4 * rows * n_slots, 0, 1}; };
+  auto list = [&](const void* p) { return Blocks{p, 4 * (Wide)batch, 0, 1}; };
+  const Blocks src[4] = {slots_of(k_src), slots_of(v_src), records(acc_src), records(pos_src)};
+  const Blocks dst[5] = {slots_of(k_dst), slots_of(v_dst), records(acc_dst), records(pos_dst), list(lens_out)};
+  const Blocks in[2] = {list(lens), list(slots)};
   const bool in_place = k_src == k_dst;
   for (int i = 0; i < 5; i++) {
     for (int j = 0; j < 4; j++) {
@@ -244,11 +255,11 @@ lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const
     for (int j = 0; j < i; j++)
       if (overlap(dst[i], dst[j])) return bad(who, "the destinations overlap one another");
   }
-  for (const Range& r : src)
+  for (const Blocks& r : src)
     if (r.p && !here(r.p)) return bad(who, ELSEWHERE);
-  for (const Range& r : dst)
+  for (const Blocks& r : dst)
     if (r.p && !here(r.p)) return bad(who, ELSEWHERE);
-  for (const Range& r : in)
+  for (const Blocks& r : in)
     if (r.p && !here(r.p)) return bad(who, ELSEWHERE);
   Evict a = {};
   a.kv_heads = (int)shape->kv_heads, a.d = (int)shape->head_dim, a.ctx = (int)shape->ctx;

@@ -51,3 +51,30 @@ def test_weights_that_repeat(cuda_lib, lens, budget, first, last, pattern, in_pl
     assert lo.cpu().tolist() == [min(n, budget) for n in lens]
     for x, w in zip(o, want):
         assert np.array_equal(x.cpu().numpy(), w)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_keys_and_values_of_a_slot_side_by_side(cuda_lib, in_place):
+    """One array [slot][K, V][kv][ctx][d]: the calls take K and V as two caches of twice the stride."""
+    import torch
+    n_slots, kv, ctx, d, lens, budget, first, last = 4, 2, 150, 64, [150, 91, 33], 40, 3, 10
+    rng = np.random.default_rng(12)
+    both = rng.integers(-32768, 32767, (n_slots, 2, kv, ctx, d), dtype=np.int16)
+    acc = rng.random((n_slots, kv, ctx)).astype(np.float32)
+    slots = [2, 0, 3]
+    want, want_acc = both.copy() if in_place else np.full_like(both, 7), acc.copy() if in_place else np.full_like(acc, 7)
+    for slot, n in zip(slots, lens):
+        for h in range(kv):
+            keep = evict_reference(acc[slot, h], n, budget, first, last)
+            want[slot, :, h, :len(keep)] = both[slot][:, h, keep]
+            want_acc[slot, h, :len(keep)] = acc[slot, h, keep]
+    src = torch.from_numpy(both).cuda(), torch.from_numpy(acc).cuda()
+    dst = src if in_place else tuple(torch.full_like(x, 7) for x in src)
+    sd, ld = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in (slots, lens))
+    lo = torch.zeros(3, dtype=torch.int32, device="cuda")
+    check(cuda_lib.lfm_cache_evict(shape_of("f16", kv, kv, d, ctx), ptr(src[0][:, 0]), ptr(src[0][:, 1]), ptr(src[1]), None,
+                                   ptr(dst[0][:, 0]), ptr(dst[0][:, 1]), ptr(dst[1]), None, 2 * kv * ctx * d, n_slots,
+                                   ptr(sd), ptr(ld), ptr(lo), 3, max(lens), budget, first, last, None), "evict")
+    assert status_of(cuda_lib) == 0
+    assert lo.cpu().tolist() == [40, 40, 33]
+    assert np.array_equal(dst[0].cpu().numpy(), want) and np.array_equal(dst[1].cpu().numpy(), want_acc)
