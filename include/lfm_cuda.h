@@ -350,10 +350,11 @@ lfm_status lfm_attention_prefill(const float* q_dev, uint32_t q_stride, const vo
  * head h / (heads / kv_heads).
  *
  * A query at position p sees position j when j <= p and (window == 0 or
- * p - j < window or j < sinks). Only positions that some query of the call
- * sees are read; a cache row that no query of the call sees may hold anything,
- * NaN included. A value that is not finite in a row that is seen spreads to
- * the queries that see it and may spread to the other queries of the call.
+ * p - j < window or j < sinks). Results depend on the positions that some query
+ * of the call sees and on no other: a cache row that none sees may hold
+ * anything, NaN included (it may be read; nothing behind a slot's ctx rows is).
+ * A value that is not finite in a row that is seen spreads to the queries that
+ * see it and may spread to the other queries of the call.
  *
  * All calls are asynchronous on `stream`, allocate nothing and may be captured
  * into a graph. Pointers are device pointers of the current device (others are
@@ -419,7 +420,9 @@ lfm_status lfm_attention_shared(const lfm_attn_shape* shape, const void* q, uint
  * exp(scale q_th.k_j - lse[t][h]), for the positions that t sees. acc
  * [kv_heads][ctx] fp32 is one slot's; lse is that of lfm_attention_window for
  * the same queries. All n queries may be given, or only the last few
- * that should choose what the cache keeps. The sums come out the same on every run. */
+ * that should choose what the cache keeps. The sums come out the same on every
+ * run. acc at positions that none of the queries sees is not written; calls that
+ * add to the same positions are ordered by their stream or by events. */
 lfm_status lfm_attention_weights(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* k_cache,
                                  uint32_t start, uint32_t n, uint32_t window, uint32_t sinks, const float* lse,
                                  float* acc, void* stream);

@@ -316,7 +316,10 @@ __global__ void __launch_bounds__((Cfg<T, D>::THREADS), 1)
       for (int r = 0; r < nranks; r++) sum += s_sum[r][tid];
     }
   }
-  if (tid < KEYS && j0 + tid < a.start + a.n) a.acc[(size_t)kh * a.ctx + j0 + tid] += sum;
+  // the record of a position that no row sees is another's
+  const int j = j0 + tid;
+  if (tid < KEYS && j < a.start + a.n && (a.window == 0 || j < a.sinks || a.start - j < a.window))
+    a.acc[(size_t)kh * a.ctx + j] += sum;
 }
 
 template <int T, int D>

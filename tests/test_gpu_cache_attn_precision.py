@@ -212,3 +212,28 @@ def test_fp32_queries_of_any_size(cuda_lib, d):
         most = limit("f32", plain, score_cut(d, s))
         for got in (acc[0, h], acc2[h]):
             assert norm_error(f64(got.cpu()), want) <= most, (sizes[h], norm_error(f64(got.cpu()), want), most)
+
+
+@pytest.mark.parametrize("kind,start,n,window_,sinks", [("f32", 300, 40, 50, 4), ("bf16", 129, 1, 1, 0),
+                                                        ("f16", 512, 128, 128, 131)])
+def test_weights_leave_the_records_that_no_query_sees(cuda_lib, kind, start, n, window_, sinks):
+    """Positions between the sinks and the first window, and behind the last query: not a bit changes (-0 stays -0)."""
+    import torch
+    heads, kv, d, ctx = 8, 2, 64, start + n + 70
+    g = torch.Generator(device="cuda").manual_seed(start)
+    qt, ct = torch_types(kind)
+    q = torch.randn(n, heads * d, generator=g, device="cuda").to(qt)
+    k, v = (torch.randn(kv, ctx, d, generator=g, device="cuda").to(ct) for _ in range(2))
+    lse = torch.zeros(n, heads, device="cuda")
+    sh = shape_of(kind, heads, kv, d, ctx)
+    check(cuda_lib.lfm_attention_window(sh, ptr(q), heads * d, ptr(k), ptr(v), start, n, window_, sinks,
+                                        ptr(torch.empty_like(q)), heads * d, ptr(lse), None), "window")
+    acc = torch.full((kv, ctx), -0.0, device="cuda")
+    check(cuda_lib.lfm_attention_weights(sh, ptr(q), heads * d, ptr(k), start, n, window_, sinks, ptr(lse), ptr(acc), None),
+          "weights")
+    assert status_of(cuda_lib) == 0
+    j = np.arange(ctx)
+    hidden = (j >= start + n) | ((j >= sinks) & (j <= start - window_))
+    got = acc.cpu().numpy()
+    assert (got.view(np.uint32)[:, hidden] == 0x80000000).all() and hidden.sum() > 70
+    assert (got[:, ~hidden] > 0).all()
