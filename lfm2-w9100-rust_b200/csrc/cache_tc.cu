@@ -525,7 +525,8 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
         for (int y = 0; y < nranks; y++) M = fmaxf(M, s_ml[y * each + k].x);
         for (int y = 0; y < nranks; y++) {
           const float2 ml = s_ml[y * each + k];
-          if (ml.x == -INFINITY) continue;  // that CTA has no part, and sent no output
+          // that CTA has no part, and sent no output (one whose scores are all NaN has: its sum is NaN)
+          if (ml.x == -INFINITY && ml.y == 0.f) continue;
           const float wt = exp2f(ml.x - M);
           const float4 q4 = *(const float4*)(so + (y * each + k) * F::STRIDE + c);
           L = fmaf(wt, ml.y, L);
