@@ -357,12 +357,12 @@ lfm_status lfm_attention_prefill(const float* q_dev, uint32_t q_stride, const vo
  * see it and may spread to the other queries of the call.
  *
  * All calls are asynchronous on `stream`, allocate nothing and may be captured
- * into a graph. Pointers are device pointers of the current device (others are
- * refused); q, out, caches and workspaces are 16-byte aligned; strides are in
- * elements and a multiple of 16 bytes. No output overlaps an input, but where a
- * call says so. What a kernel
- * finds wrong in device-side arguments it skips and reports through
- * lfm_attention_status. */
+ * into a graph (lfm_attention_status, which waits, excepted). Pointers are device
+ * pointers of the current device (others are refused); q, out, caches and
+ * workspaces are 16-byte aligned, the fp32 and int32 arrays 4-byte aligned;
+ * strides are in elements and a multiple of 16 bytes. No output overlaps an
+ * input, but where a call says so. What a kernel finds wrong in device-side
+ * arguments it skips and reports through lfm_attention_status. */
 #define LFM_ATTN_F32 0u  /* fp32 q and out over fp16 caches (the engine's) */
 #define LFM_ATTN_F16 1u  /* fp16 q, out and caches */
 #define LFM_ATTN_BF16 2u /* bf16 q, out and caches */

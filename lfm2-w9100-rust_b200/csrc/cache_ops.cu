@@ -44,6 +44,8 @@ bool here(const void* p) {
 const char* const ELSEWHERE = "the arrays must be memory of the current device";
 
 bool aligned(const void* p) { return (uintptr_t)p % 16 == 0; }
+// the 4-byte arrays (null where they may be left out)
+bool aligned4(const void* p) { return (uintptr_t)p % 4 == 0; }
 
 // null: the shape is good
 const char* shape_error(const lfm_attn_shape* s, bool caches_only) {
@@ -73,6 +75,7 @@ const char* rows_error(const lfm_attn_shape* s, const void* p, uint64_t stride) 
 const char* slots_error(const lfm_attn_shape* s, uint64_t slot_stride, uint32_t n_slots, const void* slots,
                         const void* lens, uint32_t batch, uint32_t max_len) {
   if (!lens) return "lens is null";
+  if (!aligned4(lens) || !aligned4(slots)) return "lens and slots must be 4-byte aligned";
   if (batch == 0 || batch > MAX_BATCH) return "1 <= batch <= 65535";
   if (n_slots == 0 || n_slots > 0x7fffffffu) return "n_slots must be 1 to 2^31 - 1";
   if (!slots && batch > n_slots) return "without slots, batch must be <= n_slots";
@@ -157,6 +160,7 @@ lfm_status lfm_attention_window(const lfm_attn_shape* shape, const void* q, uint
   if (lfm_status st = prompt_args(who, shape, q, q_stride, k_cache, start, n, window, sinks, &a)) return st;
   if (const char* e = rows_error(shape, out, out_stride)) return bad(who, e);
   if (!v_cache || !aligned(v_cache)) return bad(who, "the caches must be 16-byte aligned device pointers");
+  if (!aligned4(lse)) return bad(who, "lse must be 4-byte aligned");
   if (!here(q) || !here(k_cache) || !here(v_cache) || !here(out) || (lse && !here(lse))) return bad(who, ELSEWHERE);
   a.v = v_cache, a.out = out, a.out_stride = out_stride, a.lse = lse;
   return done(who, lfm::cache::window(a, (cudaStream_t)stream));
@@ -169,6 +173,7 @@ lfm_status lfm_attention_weights(const lfm_attn_shape* shape, const void* q, uin
   Prompt a;
   if (lfm_status st = prompt_args(who, shape, q, q_stride, k_cache, start, n, window, sinks, &a)) return st;
   if (!lse || !acc) return bad(who, "lse and acc must be device pointers");
+  if (!aligned4(lse) || !aligned4(acc)) return bad(who, "lse and acc must be 4-byte aligned");
   if (!here(q) || !here(k_cache) || !here(lse) || !here(acc)) return bad(who, ELSEWHERE);
   a.lse = const_cast<float*>(lse), a.acc = acc;
   return done(who, lfm::cache::weights(a, (cudaStream_t)stream));
@@ -185,6 +190,7 @@ lfm_status lfm_attention_decode(const lfm_attn_shape* shape, const void* q, uint
     return st;
   a.window = window >= max_len ? 0 : (int)window;
   a.sinks = (int)(sinks < shape->ctx ? sinks : shape->ctx);
+  if (!aligned4(acc)) return bad(who, "acc must be 4-byte aligned");
   a.acc = acc;
   if (!decode_here(a)) return bad(who, ELSEWHERE);
   return done(who, lfm::cache::decode(a, (cudaStream_t)stream));
@@ -230,6 +236,8 @@ lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const
   if (!k_src || !v_src || !k_dst || !v_dst || !aligned(k_src) || !aligned(v_src) || !aligned(k_dst) || !aligned(v_dst))
     return bad(who, "the caches must be 16-byte aligned device pointers");
   if (!acc_src || !acc_dst || !lens_out) return bad(who, "acc_src, acc_dst and lens_out must be device pointers");
+  if (!aligned4(acc_src) || !aligned4(acc_dst) || !aligned4(pos_src) || !aligned4(pos_dst) || !aligned4(lens_out))
+    return bad(who, "acc, pos and lens_out must be 4-byte aligned");
   if (!pos_src != !pos_dst) return bad(who, "pos_src and pos_dst are both given or both null");
   if (const char* e = slots_error(shape, slot_stride, n_slots, slots, lens, batch, max_len)) return bad(who, e);
   if (budget == 0 || (uint64_t)keep_first + keep_last > budget)
