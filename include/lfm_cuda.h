@@ -391,11 +391,13 @@ lfm_status lfm_attention_window(const lfm_attn_shape* shape, const void* q, uint
  * position lens[b] - 1 of slot slots[b] (slots null: slot b), whose cache
  * starts at element slots[b] * slot_stride. lens and slots are device int32;
  * 0 <= lens[b] <= max_len <= ctx, where max_len is the host's bound that sizes
- * the launch. lens[b] == 0 gives a row of zeros. acc [n_slots][kv_heads][ctx]
- * fp32 (may be null): the attention weight that each seen position got is
- * added to it, summed over the query heads of the KV head; the slots are then
- * distinct. A slot or a length out of range gives a row of zeros and is
- * reported by lfm_attention_status. batch <= 65535. */
+ * the launch. lens[b] == 0 gives a row of zeros. A slot or a length out of range
+ * gives a row of zeros and is reported by lfm_attention_status. batch <= 65535.
+ * acc [n_slots][kv_heads][ctx] fp32 (may be null): the attention weight that each
+ * seen position got is added to it, summed over the query heads of the KV head;
+ * the slots are then distinct. Whoever appends a token writes 0 to acc at its
+ * position: after an eviction, or in a slot used before, an earlier position's
+ * weight is left there. */
 lfm_status lfm_attention_decode(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* k_cache,
                                 const void* v_cache, uint64_t slot_stride, uint32_t n_slots, const int32_t* slots,
                                 const int32_t* lens, uint32_t batch, uint32_t max_len, uint32_t window,
@@ -405,9 +407,9 @@ lfm_status lfm_attention_decode(const lfm_attn_shape* shape, const void* q, uint
  * prefix_len positions of the prefix cache [kv_heads][prefix_ctx][head_dim]
  * and the lens[b] positions of its own slot (as in lfm_attention_decode,
  * lens[b] may be 0; with prefix_len 0 too the row is zeros). The prefix is
- * read once for all sessions, not once for each. `workspace` (16-byte aligned) has at least
- * lfm_attention_shared_workspace bytes; calls that overlap on the GPU, and
- * captured graphs that may, have one each. */
+ * read once for all sessions, not once for each. `workspace` (16-byte aligned)
+ * has at least lfm_attention_shared_workspace bytes; calls that overlap on the
+ * GPU, and captured graphs that may, have one each. */
 size_t lfm_attention_shared_workspace(const lfm_attn_shape* shape, uint32_t batch, uint32_t prefix_len);
 lfm_status lfm_attention_shared(const lfm_attn_shape* shape, const void* q, uint64_t q_stride, const void* prefix_k,
                                 const void* prefix_v, uint32_t prefix_ctx, uint32_t prefix_len, const void* k_cache,
@@ -437,10 +439,11 @@ lfm_status lfm_attention_weights(const lfm_attn_shape* shape, const void* q, uin
  * which are the source arrays themselves (in place; all of them then) or do
  * not overlap them (slots of K and of V may lie between one another, as in an
  * array [slot][K, V][kv_heads][ctx][head_dim]). lens_out[b] = min(lens[b], budget), in another array than
- * lens. Rows behind the kept ones are left as they were. Only dtype's cache type, kv_heads, head_dim and
- * ctx of `shape` are used. Slots are distinct: a session whose slot an earlier
- * one has, or whose slot or length is out of range, is left out and reported
- * by lfm_attention_status. batch <= 65535. */
+ * lens. Rows behind the kept ones are left as they were, acc and pos too: a token
+ * that is appended there brings its own (acc 0). Only dtype's cache type,
+ * kv_heads, head_dim and ctx of `shape` are used. Slots are distinct: a session
+ * whose slot an earlier one has, or whose slot or length is out of range, is left
+ * out (lens_out[b] too) and reported by lfm_attention_status. batch <= 65535. */
 lfm_status lfm_cache_evict(const lfm_attn_shape* shape, const void* k_src, const void* v_src, const float* acc_src,
                            const int32_t* pos_src, void* k_dst, void* v_dst, float* acc_dst, int32_t* pos_dst,
                            uint64_t slot_stride, uint32_t n_slots, const int32_t* slots, const int32_t* lens,
