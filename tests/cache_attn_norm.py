@@ -54,10 +54,12 @@ def _halves(x, keep_low):
     return hi + (x - hi).astype(np.float16).astype(np.float64) if keep_low else hi
 
 
-def emulate_f32(q, k, v, scale, q_low=True, p_low=True, shift=SHIFT["f32"]):
-    """One row of fp32 queries as the kernels' number formats have it (sums in 64 bits): q and the weights as fp16
-    pairs, of which a half can be left out, the weights relative to the maximum less `shift`."""
-    s = (k @ _halves((q * scale * LOG2E).astype(np.float32).astype(np.float64), q_low)).astype(np.float32)
+def emulate_f32(q, k, v, scale, q_low=True, p_low=True, shift=SHIFT["f32"], to_size=True):
+    """One row of fp32 queries as the kernels' number formats have it (sums in 64 bits): q, brought to size by a power
+    of two (or only times the scores' scale), and the weights as fp16 pairs, of which a half can be left out, the weights relative to the maximum less
+    `shift`."""
+    by = 2.0 ** (13 - math.floor(math.log2(np.abs(q).max()))) if to_size else scale * LOG2E
+    s = ((k @ _halves(q * by, q_low)).astype(np.float32) * np.float32(scale * LOG2E / by)).astype(np.float32)
     m = np.float32(s.max() - np.float32(shift))
     p = np.exp2((s - m).astype(np.float64)).astype(np.float32).astype(np.float64)
     return _halves(p, p_low) @ v / p.sum()

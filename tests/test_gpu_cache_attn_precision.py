@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from cache_attn_norm import SHIFT, dominated, fp16_floor, limit, norm_error, plain32, score_cut
-from cache_attn_ref import attend, ptr, torch_types
+from cache_attn_ref import attend, ptr, seen, torch_types
 from test_gpu_cache_attn import check, f64, shape_of, status_of
 
 pytestmark = pytest.mark.gpu
@@ -54,11 +54,12 @@ def shared(lib, kind, heads, q, pk, pv, k, v, lens):
     return out
 
 
-def row_errors(kind, q, k, v, got, growth=0.0):
+def row_errors(kind, q, k, v, got, growth=0.0, see=None):
     """The error in norm and its limit for rows got [heads][d] over k, v [kv][n][d]; `growth` is the power of two that
     the kernel leaves free above the largest weight (fp16 queries of many rows: 2^8)."""
     heads, d = q.shape
-    g, every = heads // len(k), np.ones(k.shape[1], bool)
+    g, every = heads // len(k), np.ones(k.shape[1], bool) if see is None else see
+    k, v, every = k[:, every], v[:, every], every[every]
     rows = [attend(q[h], k[h // g], v[h // g], every, d ** -0.5) for h in range(heads)]
     want = np.stack([r[0] for r in rows])
     floor = np.linalg.norm([fp16_floor(r[2], v[h // g], SHIFT[kind] - growth) for h, r in enumerate(rows)])
@@ -237,3 +238,48 @@ def test_weights_leave_the_records_that_no_query_sees(cuda_lib, kind, start, n, 
     got = acc.cpu().numpy()
     assert (got.view(np.uint32)[:, hidden] == 0x80000000).all() and hidden.sum() > 70
     assert (got[:, ~hidden] > 0).all()
+
+
+# The shapes of the calls in earnest, each row against the limit of its own type; a call's fp32 path that loses a half of
+# its pairs is off by 2e-4 where 2e-6 to 4e-6 are allowed.
+NORM = [  # kind, heads, kv, d, lens, window, sinks, prefix
+    ("f32", 32, 8, 64, [577, 1, 33, 2000], 0, 0, 500),
+    ("f32", 16, 8, 128, [300, 17, 128], 0, 0, 129),
+    ("f32", 6, 1, 64, [3000, 40], 1000, 40, 1),
+    ("f32", 8, 1, 128, [5000], 128, 5, 2000),
+    ("f16", 32, 8, 64, [577, 1, 33], 0, 0, 500),
+    ("f16", 12, 2, 128, [3000, 63], 700, 3, 64),
+    ("bf16", 32, 4, 128, [1100, 3, 999], 128, 5, 300),
+    ("bf16", 7, 7, 64, [90, 2048], 0, 0, 1000),
+]
+
+
+@pytest.mark.parametrize("kind,heads,kv,d,lens,window_,sinks,prefix", NORM)
+def test_errors_in_norm(cuda_lib, kind, heads, kv, d, lens, window_, sinks, prefix):
+    import torch
+    batch, ctx = len(lens), max(lens) + 5
+    g = torch.Generator(device="cuda").manual_seed(heads * d)
+    qt, ct = torch_types(kind)
+    q = (1.5 * torch.randn(batch, heads * d, generator=g, device="cuda")).to(qt)
+    k, v = (torch.randn(batch, kv, ctx, d, generator=g, device="cuda").to(ct) for _ in range(2))
+    pk, pv = (torch.randn(kv, prefix, d, generator=g, device="cuda").to(ct) for _ in range(2))
+    sh, ld = shape_of(kind, heads, kv, d, ctx), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    stepped, acc = torch.empty_like(q), torch.zeros(batch, kv, ctx, device="cuda")
+    check(cuda_lib.lfm_attention_decode(sh, ptr(q), heads * d, ptr(k), ptr(v), kv * ctx * d, batch, None, ptr(ld), batch,
+                                        max(lens), window_, sinks, ptr(acc), ptr(stepped), heads * d, None), "decode")
+    behind = shared(cuda_lib, kind, heads, q, pk, pv, k, v, lens)
+    prompt = torch.empty_like(q)
+    for b, n in enumerate(lens):  # each session's newest token as a prompt of one
+        check(cuda_lib.lfm_attention_window(sh, ptr(q[b]), heads * d, ptr(k[b]), ptr(v[b]), n - 1, 1, window_, sinks,
+                                            ptr(prompt[b]), heads * d, None, None), "window")
+    assert status_of(cuda_lib) == 0
+    q64, k64, v64, pk64, pv64 = (f64(x.cpu()) for x in (q, k, v, pk, pv))
+    growth = 8.0 if kind == "f16" else 0.0
+    for b, n in enumerate(lens):
+        see = seen(n - 1, np.arange(n), window_, sinks)
+        for out, how, least in ((stepped, see, 0.0), (prompt, see, growth), (behind, None, growth)):
+            kk, vv = k64[b, :, :n], v64[b, :, :n]
+            if how is None:
+                kk, vv = np.concatenate((pk64, kk), 1), np.concatenate((pv64, vv), 1)
+            error, most = row_errors(kind, q64[b].reshape(heads, d), kk, vv, f64(out[b].cpu()).reshape(heads, d), least, how)
+            assert error <= most, (b, out is stepped, out is prompt, error, most)
