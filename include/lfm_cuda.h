@@ -374,7 +374,7 @@ typedef struct lfm_attn_shape {
   uint32_t kv_heads; /* 1..1024 */
   uint32_t head_dim; /* 64 or 128 */
   uint32_t ctx;      /* positions of a cache slot, 1..2^24 */
-  float scale;       /* of q.k, finite and > 0; 0 means 1/sqrt(head_dim) */
+  float scale;       /* of q.k, 2^-126 to 2^127; 0 means 1/sqrt(head_dim) */
 } lfm_attn_shape;
 
 /* Prompt attention with a sliding window and sinks: queries at positions

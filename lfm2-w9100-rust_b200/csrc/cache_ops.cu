@@ -57,7 +57,9 @@ const char* shape_error(const lfm_attn_shape* s, bool caches_only) {
   if (caches_only) return nullptr;
   if (s->heads == 0 || s->heads % s->kv_heads || s->heads / s->kv_heads > LFM_ATTN_MAX_GROUP)
     return "heads must be kv_heads times 1 to 8";
-  if (!isfinite(s->scale) || s->scale < 0.f) return "scale must be finite and > 0 (0: 1/sqrt(head_dim))";
+  // the kernels take powers of two: scale * log2 e is finite too, and keeps fp32's bits
+  if (!(s->scale == 0.f || (s->scale >= 0x1p-126f && s->scale <= 0x1p127f)))
+    return "scale must be 2^-126 to 2^127 (0: 1/sqrt(head_dim))";
   return nullptr;
 }
 

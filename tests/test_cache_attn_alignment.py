@@ -1,5 +1,6 @@
-"""fp32 and int32 arrays that are not 4-byte aligned are refused (no GPU): the
-kernels read them by the word, and a misaligned address is a fault of the GPU."""
+"""Arguments at the ends of what the kernels can take (no GPU). fp32 and int32
+arrays that are not 4-byte aligned are refused: the kernels read them by the
+word, and a misaligned address is a fault of the GPU."""
 
 import pytest
 
@@ -22,3 +23,14 @@ def test_misaligned_words(call):
         assert "4-byte aligned" in _lib()[1].lfm_ops_error().decode()
     assert call(4) == 1  # aligned: refused only because these are no device pointers
     assert "current device" in _lib()[1].lfm_ops_error().decode()
+
+
+@pytest.mark.parametrize("call", [window, weights, decode, shared])
+def test_scales_whose_powers_of_two_are_no_fp32_number(call):
+    """scale * log2 e above fp32's largest, and scales below its smallest normal number."""
+    for bad in (3e38, 2.5e38, 1e-39, 1e-45):
+        assert call(sh=_shape(scale=bad)) == 1
+        assert "scale" in _lib()[1].lfm_ops_error().decode()
+    for good in (2.0 ** 127, 2.0 ** -126, 0.0, -0.0, 1.0):
+        assert call(sh=_shape(scale=good)) == 1
+        assert "current device" in _lib()[1].lfm_ops_error().decode()
