@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(THREADS, (Cfg<T, D>::CTAS))
           const float f[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
           uint32_t h[4], l[4];
           const float back = pairs<D / 8>(f, h, l);
-          if (c == 0) s_row[qr] = back * a.scale2;
+          if (c == 0) s_row[qr] = fmaxf(back * a.scale2, 0x1p-126f);  // > 0: masked scores are -inf times it
           st_piece(chunk, qr, c & 7, make_uint4(h[0], h[1], h[2], h[3]));
           st_piece(chunk + F::Q_TILE, qr, c & 7, make_uint4(l[0], l[1], l[2], l[3]));
         } else {
