@@ -12,9 +12,9 @@
 // query heads. For fp32 queries the row r + 8 holds what the fp16 row r leaves
 // off (hi/lo pairs of q and of the weights), so one instruction does both halves
 // and the sum of the two accumulator rows, which one thread holds, has ~22 bits.
-// A chunk's output is added to the running one in fp32: accumulated in the matrix
-// unit, which cuts its sums off, outputs came out smaller by 1.6e-5 of themselves
-// over 2048 positions of a warp and by 6.6e-5 over 8192.
+//   A chunk's output is added to the running one in fp32: accumulated in the
+//       matrix unit, which cuts its sums off, outputs came out smaller by 1.6e-5
+//       of themselves over 2048 positions of a warp and by 6.6e-5 over 8192.
 //   S = Q K^T: a lane reads 16 bytes of one key's row; the order of the
 //       head_dim terms that this gives the instruction's k index is the same
 //       for q, whose fragments are laid out to match. No transposed load.
@@ -22,15 +22,18 @@
 //       lane reads the same 16 bytes of 4 positions and pairs them by byte
 //       permutes; output column n of tile e is head_dim index 8 n + e.
 // Statistics and outputs stay in fp32; exponentials are of powers of two (the
-// scores carry scale * log2 e), relative to the maximum less
-// SHIFT (cache_common.cuh). 16-bit queries: the weights are rounded to the
-// caches' type, half a step each (fp16 2^-11, bf16 2^-8), as the caller's V and
-// output are; pairs would double the products. The sums l are of the weights as
-// they were. The warps join through shared
-// memory, the CTAs through the cluster's: each sends its part of the columns to
-// the CTA that finishes them, so a call is one launch without workspace. Accumulated weights need
-// the joined statistics: a CTA keeps its scores in shared memory until the
-// join, or, where they would not fit, reads K once more.
+// scores carry scale * log2 e), relative to the maximum less SHIFT
+// (cache_common.cuh). 16-bit queries: the weights are rounded to the caches'
+// type, half a step each (fp16 2^-11, bf16 2^-8), as the caller's V and output
+// are; the sums l are of the weights as they were. (Pairs in the rows that 16-bit
+// queries leave free take the error from 2.3e-4 to 2.1e-4 in fp16 and from 2.1e-3
+// to 1.6e-3 in bf16, and 24 long fp16 sessions with weights from 361 to 390 us,
+// 64 bf16 sessions of up to 4096 positions from 124 to 135 us: not taken.)
+// The warps join through shared memory, the CTAs through the cluster's: each
+// sends its part of the columns to the CTA that finishes them, so a call is one
+// launch without workspace. Accumulated weights need the joined statistics: a CTA
+// keeps its scores in shared memory until the join, or, where they would not fit,
+// reads K once more.
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -47,10 +50,12 @@ using namespace dev;
 constexpr int STAGES = 2, HALF = 4096, STAGE = 2 * HALF;
 constexpr float LOG2E = 1.4426950408889634f;
 enum Acc { NO_ACC = 0, STORED = 1, AGAIN = 2 };
-// Warps of a CTA. 4: three CTAs to an SM. 3: four, where that saves a second round (64 sessions of 1028 positions and 8
-// heads, 512 CTAs: 26 instead of 32 us; 256 sessions of 4 heads, 1024 CTAs: no gain). 7: where the scores are kept, one CTA
-// with what its ring leaves of shared memory (24 sessions of up to 32768 positions, 6 heads of 128 values to a KV head,
-// with weights: 356 us; reading K again 487 us; without weights 288 us).
+// Warps of a CTA. 4: three CTAs to an SM. 3: four, where that saves a second round, from 3 x 148 + 1 to 4 x 148 CTAs
+// without weights (64 windowed sessions of 8 heads, 512 CTAs: 24 instead of 30 us; 56 of 4096 positions, 448 CTAs: 74
+// instead of 90; 74 of 1000, 592 CTAs: 54 instead of 64; 64 of 64 positions: 11.1 instead of 10.7; 64 of 100 to 3000
+// positions, where rounds end apart anyway: 90 instead of 82). 7: where the scores are kept, one CTA with what its ring
+// leaves of shared memory (24 sessions of up to 32768 positions, 6 heads of 128 values to a KV head, with weights: 361 us;
+// before this, reading K again 487 us; without weights 295 us).
 constexpr int warps_of(int acc) { return acc == STORED ? 7 : 4; }
 constexpr int ctas_of(int warps) { return warps == 3 ? 4 : warps == 4 ? 3 : 1; }  // to an SM, by their rings
 constexpr int ring_of(int warps) { return warps * STAGES * STAGE; }
@@ -446,7 +451,7 @@ cudaError_t run(const Decode& a, const Joint& pre, cudaStream_t s) {
   const long long most = a.window ? std::min<long long>(a.max_len, (long long)a.window + a.sinks) : a.max_len;
   const int chunks = (int)((most + kc - 1) / kc);
   // As many CTAs to a KV head as fill three to an SM, each with chunks for its warps; more where that lets the scores
-  // be kept. At most 8: clusters of 16 left most SMs without a second CTA (625 us for the case above).
+  // be kept. At most 8: clusters of 16 left most SMs without a second CTA (625 instead of 487 us where K was read again).
   const int g = a.heads / a.kv_heads;
   int nranks = 1;
   // the most positions that one CTA may get, in whole chunks

@@ -11,8 +11,7 @@
 // written lies in front of everything that later rounds and passes read, since
 // the row that becomes the r-th comes from position r or behind.
 // Bound by memory, of which it reaches 83%: every kept row is read and written
-// once, but a CTA's loads wait for its stores to be issued. (The weights read from
-// memory in every pass: 172 instead of 151 us for 48 sessions.)
+// once, but a CTA's loads wait for its stores to be issued.
 #include <algorithm>
 
 #include "cache_attn.h"
@@ -25,7 +24,9 @@ using namespace dev;
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, EACH = 4, UNIT = THREADS * EACH, BINS = 2048;
 constexpr int LIST = 2048;  // positions that are listed and not yet moved: fewer than a round's 1024 and a unit's 1024
-constexpr int KEYS = 8192;  // up to so many positions' keys are read from memory once and kept
+// Up to so many positions' keys are read from memory once and kept: what static shared memory holds beside the lists.
+// Longer sessions read their weights in every pass (all of them: 172 instead of 151 us for 48 sessions of up to 8192).
+constexpr int KEYS = 8192;
 
 // A weight's order as an unsigned: larger weights have larger keys, NaN the smallest.
 __device__ __forceinline__ unsigned order_key(float x) {
@@ -230,7 +231,9 @@ cudaError_t status_word_evict(unsigned** at) { return status_word(at); }
 
 cudaError_t evict(const Evict& a, cudaStream_t s) {
   // As many CTAs to a head as give every SM two, each with a round of its own at least. More repeat the selection for
-  // less work each: 48 sessions of 8 heads cut to 2045 of up to 8192 positions 151 us with one, 159 us with two.
+  // less work each, fewer leave SMs idle. Rules of one, two and four to an SM: 16 sessions of 8 heads, 8192 to 2045
+  // positions, 66, 66 and 90 us; 24 of up to 8192 95, 82 and 101; 48 153, 153 and 163; 37 of 4 heads, 3000 to 1000,
+  // 25, 21 and 32; one of 4096 to 1024 13.8 each.
   const int rows = 8192 / a.d, most = std::min(a.max_len, a.budget);
   int nranks = 1;
   while (nranks < 8 && (long long)a.batch * a.kv_heads * nranks < 2 * 148 && rows * nranks < most) nranks *= 2;

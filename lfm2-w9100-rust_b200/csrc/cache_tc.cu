@@ -18,18 +18,22 @@
 // of which either unit was busy for half: 282 us for 8192 tokens, window 1500.)
 //
 // 16-bit queries: O stays in tensor memory, and a row's maximum is raised, and O
-// rescaled, only when it grows by more than 2^8; over long rows it is moved every FOLD tiles into
-// a running output. Weights are relative to the
-// maximum less TOP, which keeps them inside fp16's range up to that growth and
-// their roundings relative (fp16: down to 2^-21 of the largest). They are
-// rounded to the caches' type, half a step each (fp16 2^-11, bf16 2^-8), as the
-// caller's V and output are: pairs would double the second product. The sums l
-// are of the weights as they were. Together with the output's own rounding that
-// is 2.2e-3 of error in bf16 (1.6e-3 with fp32 weights). fp32 queries: q and P are fp16 hi/lo
-// pairs, two MMAs each, the low parts first; the tensor core cuts its sums off
-// instead of rounding them, a loss that grows with their number (2.2e-6 over
-// 1024 positions), so O of each tile starts from zero and is added to the
-// running output in registers.
+// rescaled, only when it grows by more than 2^8; over long rows it is moved every
+// FOLD tiles into a running output. Weights are relative to the maximum less TOP,
+// which keeps them inside fp16's range up to that growth and their roundings
+// relative (fp16: down to 2^-21 of the largest). They are rounded to the caches'
+// type, half a step each (fp16 2^-11, bf16 2^-8), as the caller's V and output
+// are; the sums l are of the weights as they were. With the output's own rounding
+// that is 2.2e-3 of error in bf16 and 2.8e-4 in fp16. (Pairs of weights and two
+// MMAs: 1.6e-3 and 2.1e-4, what the output's rounding alone leaves, for 252
+// instead of 207 us on 8192 bf16 tokens of 128 values behind a window of 1500,
+// 130 instead of 115 us on 256 bf16 sessions behind a prefix, 73 instead of 67 us
+// on 3840 fp16 tokens of 64 values: not taken.)
+// fp32 queries: q, brought to size row by row, and P are fp16 hi/lo pairs, two
+// MMAs each, the low parts first; the tensor core cuts its sums off instead of
+// rounding them, a loss that grows with their number (2.2e-6 over 1024
+// positions), so O of each tile starts from zero and is added to the running
+// output in registers. A score of s nats still loses up to head_dim / 16 * 2^-23 s.
 // Few row tiles leave SMs idle, so a cluster of CTAs may split the positions of
 // one tile; each sends its part of a row to the CTA that finishes the row.
 // Every wait is bounded; one that runs out is reported and the CTA releases

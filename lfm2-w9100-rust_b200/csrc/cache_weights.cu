@@ -12,14 +12,15 @@
 //   warps 2-17  the sums; a key is shared by four threads, each for a quarter of the columns
 //   from 18 on  the rows' lse, and for fp32 queries the tiles: fp16 hi/lo pairs, two MMAs
 // 16-bit queries are bound by the exponentials: 16 a cycle and SM, 2048 cycles for
-// a tile of 128 keys and 256 rows. 8191 bf16 tokens of 32 heads and 128 values: 345 us with the inputs in
-// L2, the special-function units busy for 80% of it, 370 us from memory. A third of
-// the exponentials through the fma units (range reduction and a polynomial of
-// degree 5) took the units' time down to 55% and left the total: the issuing warp
-// and the sums' start on each tile are what is left. Tiles of 128 rows in four buffers: 350 us;
-// eight warps for the sums: 434 us. fp32 queries are bound by making their pairs, once for each tile
-// of keys: 3840 tokens of 32 heads and 64 values 170 us with eight warps at it (four: 385 before the pairs were made two
-// pieces at a time).
+// a tile of 128 keys and 256 rows. 8191 bf16 tokens of 32 heads and 128 values:
+// 353 us with the inputs in L2, 378 us from memory, the special-function units
+// busy for 75% of it. A third of the exponentials through the fma units (range
+// reduction and a polynomial of degree 5) took the units' time down to 55% and
+// left the total: the issuing warp and the sums' start on each tile are what is
+// left. Tiles of 128 rows in four buffers were 2% slower, eight warps for the sums
+// 25%. fp32 queries are bound by making their pairs, once for each tile of keys:
+// 3840 tokens of 32 heads and 64 values 177 us, with eight warps at it (four took
+// twice that).
 // A key is summed by one thread, in the order of the rows, tile by tile, and the
 // CTAs of a cluster that splits the rows are added up in their order: the
 // result is the same on every run.
