@@ -283,3 +283,29 @@ def test_errors_in_norm(cuda_lib, kind, heads, kv, d, lens, window_, sinks, pref
                 kk, vv = np.concatenate((pk64, kk), 1), np.concatenate((pv64, vv), 1)
             error, most = row_errors(kind, q64[b].reshape(heads, d), kk, vv, f64(out[b].cpu()).reshape(heads, d), least, how)
             assert error <= most, (b, out is stepped, out is prompt, error, most)
+
+
+@pytest.mark.parametrize("kind,d", [("f16", 64), ("bf16", 128)])
+def test_many_long_rows(cuda_lib, kind, d):
+    """A prompt's chunk deep in a long cache: enough rows that each CTA walks all positions of its rows and folds, with
+    the causal edge, and the window's, in the tiles behind."""
+    import torch
+    heads, kv, n, start = 16, 2, 1200, 5000
+    g = torch.Generator(device="cuda").manual_seed(d)
+    qt, ct = torch_types(kind)
+    q = (1.5 * torch.randn(n, heads * d, generator=g, device="cuda")).to(qt)
+    k, v = (torch.randn(kv, start + n, d, generator=g, device="cuda").to(ct) for _ in range(2))
+    sh = shape_of(kind, heads, kv, d, start + n)
+    for window_, sinks in ((0, 0), (4700, 70)):
+        out = torch.full_like(q, float("nan"))
+        check(cuda_lib.lfm_attention_window(sh, ptr(q), heads * d, ptr(k), ptr(v), start, n, window_, sinks, ptr(out),
+                                            heads * d, None, None), "window")
+        assert status_of(cuda_lib) == 0
+        p, j = torch.arange(start, start + n, device="cuda")[:, None], torch.arange(start + n, device="cuda")[None]
+        see = (j <= p) & ((p - j < window_) | (j < sinks)) if window_ else j <= p
+        for h in range(heads):
+            x = q.view(n, heads, d)[:, h].double() @ k[h // 8].double().T * d ** -0.5
+            want = torch.softmax(x.masked_fill(~see, float("-inf")), -1) @ v[h // 8].double()
+            got = out.view(n, heads, d)[:, h].double()
+            error = ((got - want).norm(dim=1) / want.norm(dim=1)).max().item()
+            assert error <= limit(kind, 0.0, score_cut(d, x[see].abs().max().item())), (h, error)
